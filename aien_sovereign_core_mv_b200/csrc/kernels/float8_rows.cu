@@ -1,0 +1,430 @@
+// Numbers in 8 bits (e4m3) with one float32 scale for each block of 128: rows (a norm's, a gated activation's, any), weights
+// in blocks of 128 x 128, and the plain product of such matrices.
+//
+// A block with largest magnitude m gets the scale s = max(m / 448, 2^-126) and the codes e4m3(x * (1 / s)), to the nearest, ties to
+// even, at most 448.  A block of zeros has codes 0; a block that holds an infinity or something that is not a number has a
+// scale and codes that are not numbers, so that a product's row shows it as the product of the unscaled row would.
+// Largest magnitudes are taken over the bits of |x| as whole numbers: that order is the order of the numbers, and
+// what is not a number comes out above infinity instead of being lost.
+// Scales of rows are laid out [blocks, rows]: the products' kernels read a block's scales of neighbouring rows together.
+//
+// All of these are bound by memory, or for a few rows by latency: every number is read once, kept in registers while its block's
+// (or row's) maximum is found, and written once.
+#include "common.cuh"
+#include <cuda_fp8.h>
+
+namespace aien {
+
+constexpr int F8_BLOCK = 128;
+constexpr float F8_TOP = 448.0f, F8_LEAST = 1.17549435e-38f;      // the largest e4m3 number; 2^-126
+
+__device__ __forceinline__ uint32_t f8_bits(float v) { return __float_as_uint(fabsf(v)); }
+__device__ __forceinline__ float f8_scale(uint32_t top) {
+    return top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__fdiv_rn(__uint_as_float(top), F8_TOP), F8_LEAST);
+}
+__device__ __forceinline__ uint32_t f8_pair(float a, float b) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint2 f8_pack(const float v[8], float inv) {
+    return make_uint2(f8_pair(v[0] * inv, v[1] * inv) | f8_pair(v[2] * inv, v[3] * inv) << 16,
+                      f8_pair(v[4] * inv, v[5] * inv) | f8_pair(v[6] * inv, v[7] * inv) << 16);
+}
+// maximum over the 16 lanes that share a block
+__device__ __forceinline__ uint32_t f8_half_max(uint32_t v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// Eight numbers as one or two 16-byte loads.  __ldcg: what an earlier kernel of a chain wrote (see common.cuh).
+__device__ __forceinline__ void f8_load8(const float* p, float v[8]) {
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void f8_load8(const __nv_bfloat16* p, float v[8]) {
+    const uint4 r = __ldcg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+// ---------------------------------------------------------------- rows, and gated activations of rows
+// Where the eight numbers of a lane come from.  VEC: eight neighbours, loaded whole (every row starts on a 16-byte border and holds whole
+// eights); otherwise numbers lane, lane + 16, ... of the block, one by one.
+template <typename T, bool VEC> struct F8Plain {
+    const T* x;
+    long ld;
+    __device__ __forceinline__ void get(long t, int k0, int lane, int K, float v[8]) const {
+        const T* p = x + t * ld;
+        if (VEC) {
+            f8_load8(p + k0 + lane * 8, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k0 + j * 16 + lane < K ? ld_act(p + k0 + j * 16 + lane) : 0.f;
+        }
+    }
+};
+__device__ __forceinline__ float f8_gate(float g, float u, int gelu) {
+    const float f = gelu ? 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) : __fdividef(g, 1.0f + __expf(-g));
+    return f * u;
+}
+template <typename T, bool VEC> struct F8Gated {
+    const T* gu;
+    int group, gelu;
+    __device__ __forceinline__ void get(long t, int k0, int lane, int K, float v[8]) const {
+        const T* p = gu + t * 2 * (long)K;
+        if (VEC) {
+            const int i = k0 + lane * 8;
+            float g[8], u[8];
+            f8_load8(p + (group == 0 ? i : 2 * i), g);
+            f8_load8(p + (group == 0 ? K + i : 2 * i + 8), u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = f8_gate(g[j], u[j], gelu);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = k0 + j * 16 + lane;
+                const long gi = group == 0 ? i : (long)(i / group) * 2 * group + i % group;
+                v[j] = i < K ? f8_gate(ld_act(p + gi), ld_act(p + gi + (group == 0 ? K : group)), gelu) : 0.f;
+            }
+        }
+    }
+};
+
+template <bool VEC>
+__device__ __forceinline__ void f8_store(uint8_t* codes, int k0, int lane, int K, const float v[8], float inv) {
+    if (VEC) {
+        *reinterpret_cast<uint2*>(codes + k0 + lane * 8) = f8_pack(v, inv);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = k0 + j * 16 + lane;
+            if (k < K) codes[k] = (uint8_t)__nv_cvt_float_to_fp8(v[j] * inv, __NV_SATFINITE, __NV_E4M3);
+        }
+    }
+}
+
+// Half a warp takes a block of a row.  A CTA's 16 halves are `rows` rows times 16 / rows neighbouring blocks (rows a power of two), so
+// that the scales of a block, which lie side by side over the rows, leave together.
+template <typename SRC, bool VEC>
+__global__ void __launch_bounds__(256)
+rows_float8_kernel(SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, int rows) {
+    griddep_launch();
+    griddep_wait();
+    const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    const long t = (long)blockIdx.x * rows + half % rows;
+    const int b = blockIdx.y * (16 / rows) + half / rows, k0 = b * F8_BLOCK;
+    const bool live = t < T && k0 < K;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    const bool mine = live && (!VEC || k0 + lane * 8 < K);
+    if (mine) src.get(t, k0, lane, K, v);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, f8_bits(v[j]));
+    top = f8_half_max(top);
+    const float s = f8_scale(top), inv = __fdiv_rn(1.0f, s);
+    if (mine) f8_store<VEC>(codes + t * ldq, k0, lane, K, v, inv);
+    if (live && lane == 0) scales[(long)b * lds + t] = s;
+}
+
+template <typename SRC, bool VEC>
+static int launch_rows_float8(SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, cudaStream_t stream) {
+    const int blocks = (K + F8_BLOCK - 1) / F8_BLOCK;
+    int rows = 1;
+    while (rows < 8 && rows < T) rows *= 2;
+    const long gx = ((long)T + rows - 1) / rows, gy = ((long)blocks + 16 / rows - 1) / (16 / rows);
+    if (gy > 65535) return AIEN_E_SHAPE;
+    launch_chain(rows_float8_kernel<SRC, VEC>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, stream, src, codes, ldq, scales, lds, T, K, rows);
+    return launch_status();
+}
+
+// ---------------------------------------------------------------- the residual's sum and its norm
+// x += sum of the parts; h = x / sqrt(mean x^2 + eps) * w; codes and scales of h.  One CTA a row, the row in registers (NV times eight
+// numbers a thread) between the sum of squares and the codes; a block of 128 lies in half a warp.
+template <typename TD, int NV, int BS>
+__global__ void __launch_bounds__(BS)
+add_rmsnorm_float8_vec_kernel(float* x, const TD* delta, int nparts, size_t part_stride, const void* w, int wdt, float eps,
+                              uint8_t* codes, long ldq, float* scales, long lds, int H) {
+    __shared__ float red[32];
+    griddep_launch();
+    griddep_wait();
+    const size_t base = (size_t)blockIdx.x * H;
+    float v[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int i = (j * BS + threadIdx.x) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+        if (i < H) f8_load8(x + base + i, v[j]);
+    }
+    if (delta != nullptr) {
+#pragma unroll 2
+        for (int p = 0; p < nparts; ++p) {
+            float d[NV][8];
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int i = (j * BS + threadIdx.x) * 8;
+                if (i < H) f8_load8(delta + (size_t)p * part_stride + base + i, d[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if ((j * BS + threadIdx.x) * 8 < H) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[j][e] += d[j][e];
+                }
+        }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[j][e] * v[j][e];
+        const int i = (j * BS + threadIdx.x) * 8;
+        if (delta != nullptr && i < H) {
+            float4* o = reinterpret_cast<float4*>(x + base + i);
+            o[0] = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+            o[1] = make_float4(v[j][4], v[j][5], v[j][6], v[j][7]);
+        }
+    }
+    const float rstd = 1.0f / sqrtf(block_sum(ss, red) / (float)H + eps);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int i = (j * BS + threadIdx.x) * 8;
+        uint32_t top = 0;
+        if (i < H) {
+            float wv[8];
+            if (wdt == AIEN_DT_F32) f8_load8(reinterpret_cast<const float*>(w) + i, wv);
+            else f8_load8(reinterpret_cast<const __nv_bfloat16*>(w) + i, wv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[j][e] = v[j][e] * rstd * wv[e];
+                top = max(top, f8_bits(v[j][e]));
+            }
+        }
+        top = f8_half_max(top);
+        const float s = f8_scale(top), inv = __fdiv_rn(1.0f, s);
+        if (i < H) {
+            *reinterpret_cast<uint2*>(codes + (size_t)blockIdx.x * ldq + i) = f8_pack(v[j], inv);
+            if ((threadIdx.x & 15) == 0) scales[(long)(i / F8_BLOCK) * lds + blockIdx.x] = s;
+        }
+    }
+}
+
+// Any row: the sum goes back to memory and is read again.
+template <typename TD>
+__global__ void __launch_bounds__(512)
+add_rmsnorm_float8_kernel(float* x, const TD* delta, int nparts, size_t part_stride, const void* w, int wdt, float eps,
+                          uint8_t* codes, long ldq, float* scales, long lds, int H) {
+    __shared__ float red[32];
+    griddep_launch();
+    griddep_wait();
+    const size_t base = (size_t)blockIdx.x * H;
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < H; i += blockDim.x) {
+        float v = x[base + i];
+        if (delta != nullptr) {
+            for (int p = 0; p < nparts; ++p) v += ld_act(delta + (size_t)p * part_stride + base + i);
+            x[base + i] = v;
+        }
+        ss += v * v;
+    }
+    const float rstd = 1.0f / sqrtf(block_sum(ss, red) / (float)H + eps);       // (its barriers stand between the writes of x and the reads below)
+    const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    const int blocks = (H + F8_BLOCK - 1) / F8_BLOCK;
+    for (int b0 = 0; b0 < blocks; b0 += blockDim.x >> 4) {                       // every lane takes part in every round: the maximum is over whole halves
+        const int b = b0 + half, k0 = b * F8_BLOCK;
+        float v[8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = k0 + j * 16 + lane;
+            v[j] = k < H ? x[base + k] * rstd * ld_act_dyn(w, wdt, k) : 0.f;
+            top = max(top, f8_bits(v[j]));
+        }
+        top = f8_half_max(top);
+        const float s = f8_scale(top), inv = __fdiv_rn(1.0f, s);
+        f8_store<false>(codes + (size_t)blockIdx.x * ldq, k0, lane, H, v, inv);
+        if (lane == 0 && b < blocks) scales[(long)b * lds + blockIdx.x] = s;
+    }
+}
+
+template <typename TD>
+static int launch_add_rmsnorm_float8(float* x, const TD* delta, int nparts, size_t part_stride, const void* w, int w_dt, float eps,
+                                     uint8_t* codes, long ldq, float* scales, long lds, int T, int H, cudaStream_t stream) {
+    const bool vec = H % 8 == 0 && part_stride % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)codes & 7) == 0 &&
+                     (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)w) & 15) == 0;
+#define F8_NORM(NV, BS)                                                                                                              \
+    launch_chain(add_rmsnorm_float8_vec_kernel<TD, NV, BS>, dim3(T), dim3(BS), 0, stream, x, delta, nparts, part_stride, w, w_dt, eps, \
+                 codes, ldq, scales, lds, H)
+    if (vec && H <= 8 * 256) F8_NORM(1, 256);
+    else if (vec && H <= 8 * 512) F8_NORM(1, 512);
+    else if (vec && H <= 16 * 512) F8_NORM(2, 512);
+    else if (vec && H <= 32 * 512) F8_NORM(4, 512);
+    else
+        launch_chain(add_rmsnorm_float8_kernel<TD>, dim3(T), dim3(512), 0, stream, x, delta, nparts, part_stride, w, w_dt, eps, codes, ldq, scales, lds, H);
+#undef F8_NORM
+    return launch_status();
+}
+
+// ---------------------------------------------------------------- weights
+// A CTA takes a block of 128 x 128: 16 lanes a row of it, 16 rows at a time, the whole block in registers until its maximum is known.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+blocks_float8_kernel(const T* w, long ldw, uint8_t* codes, long ldq, float* scales, long lds, int N, int K) {
+    __shared__ uint32_t tops[8];
+    const int n0 = blockIdx.y * F8_BLOCK, k0 = blockIdx.x * F8_BLOCK;
+    const int r = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    float v[8][8];
+    uint32_t top = 0;
+    const F8Plain<T, VEC> src{w, ldw};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int n = n0 + i * 16 + r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        if (n < N && (!VEC || k0 + lane * 8 < K)) src.get(n, k0, lane, K, v[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, f8_bits(v[i][j]));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
+    const float s = f8_scale(top), inv = __fdiv_rn(1.0f, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int n = n0 + i * 16 + r;
+        if (n < N && (!VEC || k0 + lane * 8 < K)) f8_store<VEC>(codes + (long)n * ldq, k0, lane, K, v[i], inv);
+    }
+    if (threadIdx.x == 0) scales[(long)blockIdx.y * lds + blockIdx.x] = s;
+}
+
+// ---------------------------------------------------------------- the plain product
+// y[m][n] = sum over blocks b of (sum of a[m][k] w[n][k] over the block) * a_scales[b][m] * w_scales[n / 128][b], on the CUDA cores: any
+// sizes, strides and alignment.
+constexpr int F8S = 64, F8S_K = 32;
+__device__ __forceinline__ float f8_value(uint8_t c) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+}
+template <typename TC>
+__global__ void __launch_bounds__(256)
+matmul_float8_simple_kernel(const uint8_t* a, long lda, const float* sa, long lds, const uint8_t* w, long ldw, const float* sw, long ldsw,
+                            TC* out, long ldc, int M, int N, int K) {
+    __shared__ float As[F8S_K][F8S + 4], Ws[F8S_K][F8S + 4];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int m0 = blockIdx.y * F8S, n0 = blockIdx.x * F8S;
+    float acc[4][4] = {};
+    for (int b = 0; b * F8_BLOCK < K; ++b) {
+        float blk[4][4] = {};
+        for (int k0 = b * F8_BLOCK; k0 < min(K, (b + 1) * F8_BLOCK); k0 += F8S_K) {
+#pragma unroll
+            for (int i = 0; i < F8S * F8S_K / 256; ++i) {
+                const int at = threadIdx.x + i * 256, r = at / F8S_K, c = at % F8S_K;
+                As[c][r] = m0 + r < M && k0 + c < K ? f8_value(__ldcg(a + (long)(m0 + r) * lda + k0 + c)) : 0.f;
+                Ws[c][r] = n0 + r < N && k0 + c < K ? f8_value(__ldcg(w + (long)(n0 + r) * ldw + k0 + c)) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < F8S_K; ++k) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) blk[i][j] = fmaf(As[k][ty * 4 + i], Ws[k][tx * 4 + j], blk[i][j]);
+            }
+            __syncthreads();
+        }
+        const float f = n0 < N ? __ldcg(sw + (long)(n0 / F8_BLOCK) * ldsw + b) : 0.f;      // 64 columns lie in one block of rows of w
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float s = m0 + ty * 4 + i < M ? __ldcg(sa + (long)b * lds + m0 + ty * 4 + i) * f : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(blk[i][j], s, acc[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
+            if (m < M && n < N) out[(long)m * ldc + n] = from_f<TC>(acc[i][j]);
+        }
+}
+
+}  // namespace aien
+
+using namespace aien;
+
+// x [T, K] rows of float32 or bfloat16 (ldx numbers apart) to codes [T, K] (ldq bytes apart) and scales [ceil(K / 128), T] (lds numbers apart)
+AIEN_API int aien_quantize_rows_float8(const void* x, int dt, long ldx, void* codes, long ldq, float* scales, long lds, int T, int K, cudaStream_t stream) {
+    if (T <= 0) return 0;
+    if (K <= 0) return AIEN_E_SHAPE;
+    const bool ends = K % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)x & 15) == 0;
+#define F8_ROWS(TX, WHOLE)                                                                                                                      \
+    return ends && ldx % WHOLE == 0 ? launch_rows_float8<F8Plain<TX, true>, true>({(const TX*)x, ldx}, (uint8_t*)codes, ldq, scales, lds, T, K, stream) \
+                                    : launch_rows_float8<F8Plain<TX, false>, false>({(const TX*)x, ldx}, (uint8_t*)codes, ldq, scales, lds, T, K, stream)
+    if (dt == AIEN_DT_F32) F8_ROWS(float, 4);
+    if (dt == AIEN_DT_BF16) F8_ROWS(__nv_bfloat16, 8);
+#undef F8_ROWS
+    return AIEN_E_DTYPE;
+}
+
+// act(gate) * up of gate_up [T, 2K] (contiguous; group 0: gate columns first; else interleaved in runs of group), the same way
+AIEN_API int aien_swiglu_float8(const void* gu, int dt, int group, int gelu, void* codes, long ldq, float* scales, long lds, int T, int K, cudaStream_t stream) {
+    if (T <= 0) return 0;
+    if (K <= 0 || group < 0 || (group > 0 && K % group != 0)) return AIEN_E_SHAPE;
+    const bool vec = K % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)gu & 15) == 0 && (group == 0 || group == 8);
+#define F8_GATED(TX)                                                                                                                             \
+    return vec ? launch_rows_float8<F8Gated<TX, true>, true>({(const TX*)gu, group, gelu}, (uint8_t*)codes, ldq, scales, lds, T, K, stream)            \
+               : launch_rows_float8<F8Gated<TX, false>, false>({(const TX*)gu, group, gelu}, (uint8_t*)codes, ldq, scales, lds, T, K, stream)
+    if (dt == AIEN_DT_F32) F8_GATED(float);
+    if (dt == AIEN_DT_BF16) F8_GATED(__nv_bfloat16);
+#undef F8_GATED
+    return AIEN_E_DTYPE;
+}
+
+// delta: [nparts][T][H] (nparts >= 1; part_stride in numbers) or null
+AIEN_API int aien_add_rmsnorm_float8(float* x, const void* delta, int delta_dt, int nparts, size_t part_stride, const void* w, int w_dt, float eps,
+                                     void* codes, long ldq, float* scales, long lds, int T, int H, cudaStream_t stream) {
+    if (T <= 0) return 0;
+    if (H <= 0 || (delta != nullptr && nparts < 1)) return AIEN_E_SHAPE;
+    AIEN_DISPATCH_DTYPE(delta_dt, TD, return launch_add_rmsnorm_float8<TD>(x, (const TD*)delta, nparts, part_stride, w, w_dt, eps, (uint8_t*)codes, ldq,
+                                                                           scales, lds, T, H, stream));
+}
+
+// w [N, K] (ldw numbers apart) to codes [N, K] and scales [ceil(N / 128), ceil(K / 128)]
+AIEN_API int aien_quantize_blocks_float8(const void* w, int dt, long ldw, void* codes, long ldq, float* scales, long lds, int N, int K, cudaStream_t stream) {
+    if (N <= 0) return 0;
+    if (K <= 0) return AIEN_E_SHAPE;
+    const long gy = ((long)N + F8_BLOCK - 1) / F8_BLOCK;
+    if (gy > 65535) return AIEN_E_SHAPE;
+    const dim3 grid((K + F8_BLOCK - 1) / F8_BLOCK, (unsigned)gy);
+    const bool ends = K % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)w & 15) == 0;
+#define F8_BLOCKS(TX, WHOLE)                                                                                                        \
+    do {                                                                                                                            \
+        if (ends && ldw % WHOLE == 0) blocks_float8_kernel<TX, true><<<grid, 256, 0, stream>>>((const TX*)w, ldw, (uint8_t*)codes, ldq, scales, lds, N, K); \
+        else blocks_float8_kernel<TX, false><<<grid, 256, 0, stream>>>((const TX*)w, ldw, (uint8_t*)codes, ldq, scales, lds, N, K); \
+        return launch_status();                                                                                                     \
+    } while (0)
+    if (dt == AIEN_DT_F32) F8_BLOCKS(float, 4);
+    if (dt == AIEN_DT_BF16) F8_BLOCKS(__nv_bfloat16, 8);
+#undef F8_BLOCKS
+    return AIEN_E_DTYPE;
+}
+
+// a [M, K], w [N, K] codes; sa [ceil(K / 128), M] (lds numbers apart); sw [ceil(N / 128), ceil(K / 128)] (ldsw numbers apart); out [M, N]
+AIEN_API int aien_matmul_float8(const void* a, long lda, const float* sa, long lds, const void* w, long ldw, const float* sw, long ldsw,
+                                void* out, int c_dt, long ldc, int M, int N, int K, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (K <= 0) return AIEN_E_SHAPE;
+    const dim3 grid((N + F8S - 1) / F8S, (M + F8S - 1) / F8S);
+    if (grid.y > 65535) return AIEN_E_SHAPE;
+    AIEN_DISPATCH_DTYPE(c_dt, TC, (matmul_float8_simple_kernel<TC><<<grid, 256, 0, stream>>>((const uint8_t*)a, lda, sa, lds, (const uint8_t*)w, ldw, sw, ldsw,
+                                                                                             (TC*)out, ldc, M, N, K)));
+    return launch_status();
+}

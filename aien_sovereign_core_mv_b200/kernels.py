@@ -2451,3 +2451,142 @@ def matrix_memory_chunked(proj: torch.Tensor, q_off: int, k_off: int, v_off: int
                                             state, state.stride(0), slot_map, q_start, positions, weight, dt(weight), float(eps),
                                             float(den_eps), out, out.stride(0), scratch, T, int(num_seqs), int(heads), int(dim), int(vdim),
                                             _stream()), "matrix_memory_chunked")
+
+
+# ---------------------------------------------------------------------------- linear layers in 8 bits
+# Numbers in 8 bits are e4m3 codes with one float32 scale for each block of 128: of a row's 128 neighbours, or of 128 x 128 numbers of a
+# weight.  scale = max|x| / 448, at least 2^-126; code = e4m3(x / scale), to the nearest (the reciprocal of the scale is rounded to
+# float32 first), at most 448.  A block that holds an infinity or something that is not a number has a scale and codes that are not
+# numbers.  Codes [rows, K] may have a row stride; a last block may be short.  Scales of rows are laid out [ceil(K / 128), rows],
+# scales of a weight [ceil(N / 128), ceil(K / 128)]; both may have a row stride.
+FLOAT8_BLOCK = 128
+
+
+def float8_blocks(n: int) -> int:
+    """Blocks of 128 that n numbers fill, the last of them perhaps in part."""
+    return (int(n) + FLOAT8_BLOCK - 1) // FLOAT8_BLOCK
+
+
+def _refuse(name: str, why: str) -> None:
+    raise KernelError(f"{name}: {why}")
+
+
+def _rows_of(name: str, what: str, t: torch.Tensor, shape: tuple, dtypes: tuple) -> None:
+    """``t`` is a matrix of this shape and one of these dtypes, its rows whole and not overlapping."""
+    if t.dtype not in dtypes:
+        _refuse(name, f"{what} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)}")
+    if tuple(t.shape) != shape:
+        _refuse(name, f"{what} has shape {tuple(t.shape)}, not {shape}")
+    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        _refuse(name, f"{what} has strides {tuple(t.stride())}: its rows must be whole and apart")
+
+
+def _here(name: str, *ts: Optional[torch.Tensor]) -> None:
+    """Every tensor lives on the device that the launch goes to."""
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _refuse(name, "arguments must live on the CUDA device (there is no CPU path)")
+        if t.get_device() != torch.cuda.current_device():
+            _refuse(name, f"an argument lives on device {t.get_device()}, the launch would go to device {torch.cuda.current_device()}")
+
+
+_E4M3 = (torch.float8_e4m3fn,)
+_F32 = (torch.float32,)
+_F32_BF16 = (torch.float32, torch.bfloat16)
+
+
+def _float8_result(name: str, codes: torch.Tensor, scales: torch.Tensor, T: int, width: int) -> None:
+    if width < 1:
+        _refuse(name, "rows of no numbers")
+    _rows_of(name, "codes", codes, (T, width), _E4M3)
+    _rows_of(name, "scales", scales, (float8_blocks(width), T), _F32)
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Numbers between a matrix's rows; of a single row, its length."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def quantize_rows_float8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """x [T, K] float32 or bfloat16 (row stride free) in 8 bits: codes [T, K] e4m3, scales [ceil(K / 128), T] float32."""
+    T, width = codes.shape
+    _rows_of("quantize_rows_float8", "x", x, (T, width), _F32_BF16)
+    _float8_result("quantize_rows_float8", codes, scales, T, width)
+    _here("quantize_rows_float8", x, codes, scales)
+    _check(lib().aien_quantize_rows_float8(x, dt(x), _ld(x), codes, _ld(codes), scales, _ld(scales), T, width, _stream()), "quantize_rows_float8")
+
+
+def swiglu_float8(gate_up: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: int = 0, act: str = "silu") -> None:
+    """:func:`swiglu` with its result in 8 bits: act(gate) * up of gate_up [T, 2K], float32 or bfloat16, contiguous, computed in float32,
+    as codes [T, K] and scales [ceil(K / 128), T]."""
+    T, width = codes.shape
+    name = "swiglu_float8"
+    if act not in GATED_ACTS:
+        _refuse(name, f"activation {act!r}: known are {sorted(GATED_ACTS)}")
+    if group < 0 or (group > 0 and width % group):
+        _refuse(name, f"{width} columns do not divide into runs of {group}")
+    if not gate_up.is_contiguous():
+        _refuse(name, "gate_up must be contiguous")
+    _rows_of(name, "gate_up", gate_up, (T, 2 * width), _F32_BF16)
+    _float8_result(name, codes, scales, T, width)
+    _here(name, gate_up, codes, scales)
+    _check(lib().aien_swiglu_float8(gate_up, dt(gate_up), int(group), 1 if act == "gelu_tanh" else 0, codes, _ld(codes), scales, _ld(scales), T, width,
+                                    _stream()), name)
+
+
+def add_rmsnorm_float8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """:func:`add_rmsnorm` with its result in 8 bits: x [T, H] float32 += delta (when given: [T, H] in any kernel dtype, or float32 partial
+    products [P, T, H]) in place; rmsnorm(x) * weight as codes [T, H] and scales [ceil(H / 128), T]."""
+    T, H = codes.shape
+    name = "add_rmsnorm_float8"
+    if not x.is_contiguous():
+        _refuse(name, "x must be contiguous")
+    _rows_of(name, "x", x, (T, H), _F32)
+    nparts, stride = 1, 0
+    if delta is not None:
+        if delta.dim() == 3 and delta.dtype == torch.float32 and delta.shape[0] >= 1 and delta.is_contiguous():
+            nparts, stride = delta.shape[0], T * H
+            _rows_of(name, "delta", delta.view(nparts * T, H), (nparts * T, H), _F32)
+        else:
+            if not delta.is_contiguous():
+                _refuse(name, "delta must be contiguous")
+            _rows_of(name, "delta", delta, (T, H), _F32_BF16)
+    if weight.numel() != H or not weight.is_contiguous() or weight.dtype not in _F32_BF16:
+        _refuse(name, f"weight must be {H} contiguous numbers, float32 or bfloat16")
+    _float8_result(name, codes, scales, T, H)
+    _here(name, x, delta, weight, codes, scales)
+    _check(lib().aien_add_rmsnorm_float8(x, delta, dt(delta) if delta is not None else F32, nparts, stride, weight, dt(weight), float(eps),
+                                         codes, _ld(codes), scales, _ld(scales), T, H, _stream()), name)
+
+
+def quantize_blocks_float8(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """A weight w [N, K] float32 or bfloat16 (row stride free) in 8 bits: codes [N, K] e4m3, scales [ceil(N / 128), ceil(K / 128)] float32."""
+    N, width = codes.shape
+    name = "quantize_blocks_float8"
+    if width < 1:
+        _refuse(name, "rows of no numbers")
+    _rows_of(name, "w", w, (N, width), _F32_BF16)
+    _rows_of(name, "codes", codes, (N, width), _E4M3)
+    _rows_of(name, "scales", scales, (float8_blocks(N), float8_blocks(width)), _F32)
+    _here(name, w, codes, scales)
+    _check(lib().aien_quantize_blocks_float8(w, dt(w), _ld(w), codes, _ld(codes), scales, _ld(scales), N, width, _stream()), name)
+
+
+def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> None:
+    """out [M, N] (bfloat16 or float32, row stride free) = a . w^T of rows a [M, K] with scales [ceil(K / 128), M] and a weight w [N, K] with scales
+    [ceil(N / 128), ceil(K / 128)]: a block's sum of code products times its two scales, the blocks added up in float32."""
+    name = "matmul_float8"
+    M, N = out.shape
+    width = a.shape[-1]
+    if width < 1:
+        _refuse(name, "rows of no numbers")
+    _rows_of(name, "a", a, (M, width), _E4M3)
+    _rows_of(name, "a_scales", a_scales, (float8_blocks(width), M), _F32)
+    _rows_of(name, "w", w, (N, width), _E4M3)
+    _rows_of(name, "w_scales", w_scales, (float8_blocks(N), float8_blocks(width)), _F32)
+    _rows_of(name, "out", out, (M, N), _F32_BF16)
+    _here(name, a, a_scales, w, w_scales, out)
+    _check(lib().aien_matmul_float8(a, _ld(a), a_scales, _ld(a_scales), w, _ld(w), w_scales, _ld(w_scales), out, dt(out), _ld(out), M, N, width,
+                                    _stream()), name)
