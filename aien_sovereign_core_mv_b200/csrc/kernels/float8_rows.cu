@@ -13,6 +13,9 @@
 #include "common.cuh"
 #include <cuda_fp8.h>
 
+extern "C" int aien_matmul_float8_tc(const void* a, long lda, const float* sa, long lds, const void* w, long ldw, const float* sw, long ldsw,
+                                     void* out, int c_dt, long ldc, int M, int N, int K, cudaStream_t stream);     // gemm_float8.cuh
+
 namespace aien {
 
 constexpr int F8_BLOCK = 128;
@@ -422,6 +425,8 @@ AIEN_API int aien_matmul_float8(const void* a, long lda, const float* sa, long l
                                 void* out, int c_dt, long ldc, int M, int N, int K, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) return AIEN_E_SHAPE;
+    const bool aligned = (((uintptr_t)a | (uintptr_t)w) & 15) == 0 && (M == 1 || lda % 16 == 0) && (N == 1 || ldw % 16 == 0);
+    if (aligned) return aien_matmul_float8_tc(a, lda, sa, lds, w, ldw, sw, ldsw, out, c_dt, ldc, M, N, K, stream);
     const dim3 grid((N + F8S - 1) / F8S, (M + F8S - 1) / F8S);
     if (grid.y > 65535) return AIEN_E_SHAPE;
     AIEN_DISPATCH_DTYPE(c_dt, TC, (matmul_float8_simple_kernel<TC><<<grid, 256, 0, stream>>>((const uint8_t*)a, lda, sa, lds, (const uint8_t*)w, ldw, sw, ldsw,

@@ -1289,6 +1289,8 @@ AIEN_API int aien_gemm_tc_grouped(const void* A, long lda, const void* W, long l
     return AIEN_E_SHAPE;
 }
 
+#include "gemm_float8.cuh"
+
 // Reads and clears the error code a bounded wait may have left (0: none; 1 producer, 2 MMA, 3 epilogue).
 AIEN_API int aien_gemm_tc_error(void) {
     int v = 0, zero = 0;
