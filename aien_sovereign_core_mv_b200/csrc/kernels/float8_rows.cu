@@ -1,5 +1,5 @@
-// Numbers in 8 bits (e4m3) with one float32 scale for each block of 128: rows (a norm's, a gated activation's, any), weights
-// in blocks of 128 x 128, and the plain product of such matrices.
+// Numbers in 8 bits (e4m3) with one float32 scale for each block of 128: rows (a norm's, a gated activation's, any) and weights
+// in blocks of 128 x 128.
 //
 // A block with largest magnitude m gets the scale s = max(m / 448, 2^-126) and the codes e4m3(x * (1 / s)), to the nearest, ties to
 // even, at most 448.  A block of zeros has codes 0; a block that holds an infinity or something that is not a number has a
@@ -12,9 +12,6 @@
 // (or row's) maximum is found, and written once.
 #include "common.cuh"
 #include <cuda_fp8.h>
-
-extern "C" int aien_matmul_float8_tc(const void* a, long lda, const float* sa, long lds, const void* w, long ldw, const float* sw, long ldsw,
-                                     void* out, int c_dt, long ldc, int M, int N, int K, cudaStream_t stream);     // gemm_float8.cuh
 
 namespace aien {
 
@@ -308,57 +305,6 @@ blocks_float8_kernel(const T* w, long ldw, uint8_t* codes, long ldq, float* scal
     if (threadIdx.x == 0) scales[(long)blockIdx.y * lds + blockIdx.x] = s;
 }
 
-// ---------------------------------------------------------------- the plain product
-// y[m][n] = sum over blocks b of (sum of a[m][k] w[n][k] over the block) * a_scales[b][m] * w_scales[n / 128][b], on the CUDA cores: any
-// sizes, strides and alignment.
-constexpr int F8S = 64, F8S_K = 32;
-__device__ __forceinline__ float f8_value(uint8_t c) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-}
-template <typename TC>
-__global__ void __launch_bounds__(256)
-matmul_float8_simple_kernel(const uint8_t* a, long lda, const float* sa, long lds, const uint8_t* w, long ldw, const float* sw, long ldsw,
-                            TC* out, long ldc, int M, int N, int K) {
-    __shared__ float As[F8S_K][F8S + 4], Ws[F8S_K][F8S + 4];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int m0 = blockIdx.y * F8S, n0 = blockIdx.x * F8S;
-    float acc[4][4] = {};
-    for (int b = 0; b * F8_BLOCK < K; ++b) {
-        float blk[4][4] = {};
-        for (int k0 = b * F8_BLOCK; k0 < min(K, (b + 1) * F8_BLOCK); k0 += F8S_K) {
-#pragma unroll
-            for (int i = 0; i < F8S * F8S_K / 256; ++i) {
-                const int at = threadIdx.x + i * 256, r = at / F8S_K, c = at % F8S_K;
-                As[c][r] = m0 + r < M && k0 + c < K ? f8_value(__ldcg(a + (long)(m0 + r) * lda + k0 + c)) : 0.f;
-                Ws[c][r] = n0 + r < N && k0 + c < K ? f8_value(__ldcg(w + (long)(n0 + r) * ldw + k0 + c)) : 0.f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < F8S_K; ++k) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) blk[i][j] = fmaf(As[k][ty * 4 + i], Ws[k][tx * 4 + j], blk[i][j]);
-            }
-            __syncthreads();
-        }
-        const float f = n0 < N ? __ldcg(sw + (long)(n0 / F8_BLOCK) * ldsw + b) : 0.f;      // 64 columns lie in one block of rows of w
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float s = m0 + ty * 4 + i < M ? __ldcg(sa + (long)b * lds + m0 + ty * 4 + i) * f : 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(blk[i][j], s, acc[i][j]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m < M && n < N) out[(long)m * ldc + n] = from_f<TC>(acc[i][j]);
-        }
-}
-
 }  // namespace aien
 
 using namespace aien;
@@ -418,18 +364,4 @@ AIEN_API int aien_quantize_blocks_float8(const void* w, int dt, long ldw, void* 
     if (dt == AIEN_DT_BF16) F8_BLOCKS(__nv_bfloat16, 8);
 #undef F8_BLOCKS
     return AIEN_E_DTYPE;
-}
-
-// a [M, K], w [N, K] codes; sa [ceil(K / 128), M] (lds numbers apart); sw [ceil(N / 128), ceil(K / 128)] (ldsw numbers apart); out [M, N]
-AIEN_API int aien_matmul_float8(const void* a, long lda, const float* sa, long lds, const void* w, long ldw, const float* sw, long ldsw,
-                                void* out, int c_dt, long ldc, int M, int N, int K, cudaStream_t stream) {
-    if (M <= 0 || N <= 0) return 0;
-    if (K <= 0) return AIEN_E_SHAPE;
-    const bool aligned = (((uintptr_t)a | (uintptr_t)w) & 15) == 0 && (M == 1 || lda % 16 == 0) && (N == 1 || ldw % 16 == 0);
-    if (aligned) return aien_matmul_float8_tc(a, lda, sa, lds, w, ldw, sw, ldsw, out, c_dt, ldc, M, N, K, stream);
-    const dim3 grid((N + F8S - 1) / F8S, (M + F8S - 1) / F8S);
-    if (grid.y > 65535) return AIEN_E_SHAPE;
-    AIEN_DISPATCH_DTYPE(c_dt, TC, (matmul_float8_simple_kernel<TC><<<grid, 256, 0, stream>>>((const uint8_t*)a, lda, sa, lds, (const uint8_t*)w, ldw, sw, ldsw,
-                                                                                             (TC*)out, ldc, M, N, K)));
-    return launch_status();
 }

@@ -9,8 +9,9 @@
 // Two forms.  float8_few_kernel, for few rows of a: W's rows are the tensor memory's lanes (the M of the instruction) and the
 // tokens its columns, so that a tile of W is 128 rows whatever the number of tokens; what bounds it is W's way through memory, so as many
 // stages as fit are on their way, two CTAs on an SM, and a cluster of CTAs shares a tile's K where tiles are few.
-// float8_tiles_kernel, for many: persistent, tokens are the lanes, tiles of 128 x BN; what bounds it is the tensor cores' rate.
-// Rows and columns beyond the matrices are zero-filled by TMA, stores are masked.  Codes start on 16-byte borders, row by row.
+// float8_tiles_kernel, for many: persistent, tokens are the lanes, tiles of 128 x 128, or 256 x 256 by a pair of CTAs; what bounds it is the tensor cores' rate.
+// Rows and columns beyond the matrices are zero-filled by TMA, stores are masked.  Rows of codes that do not all start on 16-byte borders
+// are brought by threads in TMA's place (f8_gather).
 #pragma once
 #include "tma.cuh"
 #include "umma.cuh"
@@ -29,6 +30,19 @@ inline bool f8_make_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64
     cuuint32_t estr[2] = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The result [rows, cols], ld numbers between rows, in boxes of 32 rows x 128 bytes that a warp stores.
+template <typename TC>
+inline bool f8_make_map_out(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {ld * sizeof(TC)};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / sizeof(TC)), 32};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(map, sizeof(TC) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 struct F8Scales {
@@ -56,31 +70,76 @@ __device__ __forceinline__ float2 f8_split(uint64_t v) {
 }
 __device__ __forceinline__ void f8_named_barrier(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 
+__device__ __forceinline__ float4 f8_lds4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+// lane 0 arrives, without a branch
+__device__ __forceinline__ void f8_arrive0(uint32_t bar, int lane) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar), "r"(lane) : "memory");
+}
+__device__ __forceinline__ void f8_arrive0_cluster(uint32_t bar, int lane) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar), "r"(lane) : "memory");
+}
+
+// A place in a ring of N and the parity of the round that it is in.
+template <int N> struct F8Ring {
+    uint32_t at = 0, parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) { at = 0; parity ^= 1; }
+    }
+};
+
+__device__ __forceinline__ bool f8_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// mbar_wait for a barrier that the other CTA of a pair arrives at too
+__device__ __forceinline__ void f8_wait_cluster(uint32_t bar, uint32_t parity, int code) {
+    for (uint32_t i = 0; i < TC_SPIN_LIMIT; ++i) {
+        if (f8_try_wait_cluster(bar, parity)) return;
+        if ((i & 0xFFFFFu) == 0xFFFFFu && *reinterpret_cast<volatile int*>(&g_wait_error) != 0) return;
+    }
+    atomicCAS(&g_wait_error, 0, code);
+}
+
+// bytes of this CTA's shared memory to another one's of the cluster, which counts at a barrier there
+__device__ __forceinline__ void f8_copy_to_rank(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 // ---------------------------------------------------------------- few rows of a
 template <int NT> struct F8Few {
     static constexpr int STAGE_W = 128 * F8_KB, STAGE_A = NT * F8_KB;
-    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : 4;            // two CTAs on an SM: at most 113 KB each
+    static constexpr int STAGES = NT == 64 ? 3 : NT == 32 ? 4 : 5;            // two CTAs on an SM: at most 113 KB each
+    static constexpr int PARTS = NT * 128 * 4;                                // what the CTAs of a cluster send each other
     static constexpr int BUFS = 4, TMEM_COLS = BUFS * NT;                     // 64, 128 or 256 of 512 columns
-    static constexpr int CHUNK = 32;                                          // k-blocks whose scales lie ready at a time
+    static constexpr int CHUNK = NT == 64 ? 16 : 32;                          // k-blocks whose scales lie ready at a time
     static constexpr int FACTORS = CHUNK * NT * 4;
-    static constexpr int SMEM = STAGES * (STAGE_W + STAGE_A) + FACTORS + 1024 /*align*/ + 256 /*barriers*/;
+    static constexpr int SMEM = STAGES * (STAGE_W + STAGE_A) + PARTS + FACTORS + 1024 /*align*/ + 256 /*barriers*/;
 };
 
 // blockIdx.x: the CTA's rank in the cluster (gridDim.x CTAs) that shares a tile's K; y: tile of NT tokens; z: tile of 128 rows of W.
 template <int NT, typename TC>
 __global__ void __launch_bounds__(192, 2)
 float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, F8Scales sc, TC* __restrict__ out, long ldc,
-                  int M, int N, int K) {
+                  int M, int N, int K, int w_ready) {
     using C = F8Few<NT>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t sW = base, sA = base + C::STAGES * C::STAGE_W;
-    float* factors = reinterpret_cast<float*>(gen + C::STAGES * (C::STAGE_W + C::STAGE_A));
-    const uint32_t bars = base + C::STAGES * (C::STAGE_W + C::STAGE_A) + C::FACTORS;
-    const uint32_t full0 = bars, empty0 = full0 + 8 * C::STAGES, tfull0 = empty0 + 8 * C::STAGES, tempty0 = tfull0 + 8 * C::BUFS, slot = tempty0 + 8 * C::BUFS;
+    const uint32_t sParts = base + C::STAGES * (C::STAGE_W + C::STAGE_A);
+    float* factors = reinterpret_cast<float*>(gen + C::STAGES * (C::STAGE_W + C::STAGE_A) + C::PARTS);
+    const uint32_t bars = sParts + C::PARTS + C::FACTORS;
+    const uint32_t full0 = bars, empty0 = full0 + 8 * C::STAGES, tfull0 = empty0 + 8 * C::STAGES, tempty0 = tfull0 + 8 * C::BUFS, parts_in = tempty0 + 8 * C::BUFS,
+                   slot = parts_in + 8;
     volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(gen + (slot - base));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;       // (known to be the same for the whole warp)
     const int rank = blockIdx.x, Z = gridDim.x, m0 = blockIdx.y * NT, n0 = blockIdx.z * 128;
     const int total = (K + F8_KB - 1) / F8_KB;
     const int kb0 = (int)((long)total * rank / Z), num = (int)((long)total * (rank + 1) / Z) - kb0;
@@ -88,6 +147,10 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
         for (int b = 0; b < C::BUFS; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 4); }
+        mbar_init(parts_in, 1);
+        if (Z > 1) mbar_expect_tx(parts_in, (Z - 1) * (C::PARTS / Z));
+        prefetch_map(&map_w);
+        prefetch_map(&map_a);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -99,6 +162,7 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *slot_ptr;
     griddep_launch();                                                         // behind the allocation: what starts now cannot take these columns and wait for this kernel
+    if (Z > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");          // this CTA runs and its barriers are there
     const int pt = threadIdx.x - 64;                                          // of the 128 threads that add up
     const int row = (warp & 3) * 32 + lane;                                   // the tensor memory's lane
     uint64_t acc[NT / 2];
@@ -106,52 +170,66 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     for (int i = 0; i < NT / 2; ++i) acc[i] = 0;
 
     if (warp == 0) {
-        if (lane == 0) {
-            griddep_wait();
-            for (int kb = 0; kb < num; ++kb) {
-                const int s = kb % C::STAGES, round = kb / C::STAGES;
-                if (round > 0) mbar_wait(empty0 + 8 * s, (round - 1) & 1, 1);
-                mbar_expect_tx(full0 + 8 * s, C::STAGE_W + C::STAGE_A);
-                tma_load_2d(sW + s * C::STAGE_W, &map_w, full0 + 8 * s, (kb0 + kb) * F8_KB, n0);
-                tma_load_2d(sA + s * C::STAGE_A, &map_a, full0 + 8 * s, (kb0 + kb) * F8_KB, m0);
+        // W's first stages are requested ahead of the wait for the kernel before this one where the caller says that W was there before it
+        const int ahead = w_ready ? min(num, C::STAGES) : 0;
+        if (elect_one()) {
+            for (int kb = 0; kb < ahead; ++kb) {
+                mbar_expect_tx(full0 + 8 * kb, C::STAGE_W + C::STAGE_A);
+                tma_load_2d(sW + kb * C::STAGE_W, &map_w, full0 + 8 * kb, (kb0 + kb) * F8_KB, n0);
             }
         }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = umma_idesc_e4m3(128, NT);
-            for (int kb = 0; kb < num; ++kb) {
-                const int s = kb % C::STAGES, b = kb % C::BUFS, use = kb / C::BUFS;
-                mbar_wait(full0 + 8 * s, (kb / C::STAGES) & 1, 2);
-                if (use > 0) mbar_wait(tempty0 + 8 * b, (use - 1) & 1, 2);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t dw = make_desc_sw128(sW + s * C::STAGE_W), da = make_desc_sw128(sA + s * C::STAGE_A);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) umma_f8(tmem + b * NT, dw + 2 * k, da + 2 * k, idesc, k > 0 ? 1u : 0u);      // 32 codes = 2 descriptor units
-                umma_commit(empty0 + 8 * s);
-                umma_commit(tfull0 + 8 * b);
+        __syncwarp();
+        griddep_wait();
+        F8Ring<C::STAGES> r;
+        for (int kb = 0; kb < num; ++kb, r.next()) {
+            mbar_wait(empty0 + 8 * r.at, r.parity ^ 1, 1);                    // (passes at once in the first round)
+            if (elect_one()) {
+                if (kb >= ahead) {
+                    mbar_expect_tx(full0 + 8 * r.at, C::STAGE_W + C::STAGE_A);
+                    tma_load_2d(sW + r.at * C::STAGE_W, &map_w, full0 + 8 * r.at, (kb0 + kb) * F8_KB, n0);
+                }
+                tma_load_2d(sA + r.at * C::STAGE_A, &map_a, full0 + 8 * r.at, (kb0 + kb) * F8_KB, m0);
             }
+            __syncwarp();
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = umma_idesc_e4m3(128, NT);
+        const uint64_t dw0 = make_desc_sw128(sW), da0 = make_desc_sw128(sA);
+        F8Ring<C::STAGES> r;
+        F8Ring<C::BUFS> t;
+        for (int kb = 0; kb < num; ++kb, r.next(), t.next()) {
+            const uint64_t dw = dw0 + r.at * (C::STAGE_W >> 4), da = da0 + r.at * (C::STAGE_A >> 4);
+            mbar_wait(full0 + 8 * r.at, r.parity, 2);
+            mbar_wait(tempty0 + 8 * t.at, t.parity ^ 1, 2);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_f8(tmem + t.at * NT, dw + 2 * k, da + 2 * k, idesc, k > 0 ? 1u : 0u);        // 32 codes = 2 descriptor units
+                umma_commit(tfull0 + 8 * t.at);
+                umma_commit(empty0 + 8 * r.at);
+            }
+            __syncwarp();
         }
     } else {
         griddep_wait();
-        for (int kb = 0; kb < num; ++kb) {
+        F8Ring<C::BUFS> t;
+        for (int kb = 0; kb < num; ++kb, t.next()) {
             if (kb % C::CHUNK == 0) {
                 if (kb > 0) f8_named_barrier(128);                            // everyone is through with the scales before these
                 const int count = min(C::CHUNK, num - kb) * NT;
                 for (int i = pt; i < count; i += 128) {
-                    const int b = kb0 + kb + i / NT, t = m0 + i % NT;
-                    factors[i] = t < M ? __ldcg(sc.a + (long)b * sc.lda + t) * __ldcg(sc.w + (long)blockIdx.z * sc.ldw + b) : 0.f;
+                    const int b = kb0 + kb + i / NT, m = m0 + i % NT;
+                    factors[i] = m < M ? __ldcg(sc.a + (long)b * sc.lda + m) * __ldcg(sc.w + (long)blockIdx.z * sc.ldw + b) : 0.f;
                 }
                 f8_named_barrier(128);
             }
-            const int b = kb % C::BUFS;
-            mbar_wait(tfull0 + 8 * b, (kb / C::BUFS) & 1, 3);
+            mbar_wait(tfull0 + 8 * t.at, t.parity, 3);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            __syncwarp();
             const ulonglong2* f = reinterpret_cast<const ulonglong2*>(factors + (kb % C::CHUNK) * NT);
 #pragma unroll
             for (int c0 = 0; c0 < NT; c0 += 16) {
                 uint32_t r[16];
-                tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(b * NT + c0), r);
+                tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(t.at * NT + c0), r);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -162,7 +240,7 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(tempty0 + 8 * b);
+            f8_arrive0(tempty0 + 8 * t.at, lane);
         }
     }
     const int n = n0 + row;
@@ -176,31 +254,39 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
         }
     } else {
-        // Every CTA of the cluster has its part of K behind it: the rings are free.  CTA z takes columns z * NT / Z .. of everyone's
-        // sums ([rank][column][row] in its ring) and adds them up in the order of K.
-        __syncwarp();
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // CTA z takes columns z * NT / Z .. of everyone's sums and adds them up in the order of K.  They lie by owner in the ring, whose
+        // last stage has been multiplied, [owner][column][row]; one copy a CTA brings them to [from][column][row] in the owner's place for them.
+        // (Stored over the cluster number by number they took 2 us.)
         const int cw = NT / Z;
+        const uint32_t piece = C::PARTS / Z;
         if (warp >= 2) {
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
                 const float2 v = f8_split(acc[c / 2]);
-                const uint32_t to = tc_map_rank(base + (uint32_t)(((rank * cw + c % cw) * 128 + row) * 4), (uint32_t)(c / cw));
-                asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(__float_as_uint(c & 1 ? v.y : v.x)) : "memory");
+                reinterpret_cast<float*>(gen)[c * 128 + row] = c & 1 ? v.y : v.x;
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            f8_named_barrier(128);
         }
         __syncwarp();
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // everyone runs
+        if (warp == 2 && elect_one()) {
+            for (int z = 0; z < Z; ++z)
+                if (z != rank) f8_copy_to_rank(tc_map_rank(sParts + rank * piece, z), base + z * piece, piece, tc_map_rank(parts_in, z));
+        }
+        __syncwarp();
+        if (warp >= 2) f8_wait_cluster(parts_in, 0, 3);
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); // what others sent has arrived: when everyone says so, everyone may leave
         if (warp >= 2 && n < N) {
-            const volatile float* part = reinterpret_cast<const volatile float*>(gen);
             for (int c = 0; c < cw && m0 + rank * cw + c < M; ++c) {
                 float v = 0.f;
-                for (int z = 0; z < Z; ++z) v += part[(z * cw + c) * 128 + row];
+                for (int z = 0; z < Z; ++z)
+                    v += reinterpret_cast<const volatile float*>(z == rank ? gen + z * piece : gen + (sParts - base) + z * piece)[c * 128 + row];
                 out[(long)(m0 + rank * cw + c) * ldc + n] = from_f<TC>(v);
             }
         }
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -211,140 +297,350 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 }
 
 // ---------------------------------------------------------------- many rows of a
-template <int BN> struct F8Tiles {
-    static constexpr int STAGE_A = 128 * F8_KB, STAGE_W = BN * F8_KB;
-    static constexpr int STAGES = 192 * 1024 / (STAGE_A + STAGE_W);           // 4 of 48 KB, 6 of 32 KB
+// The scales' way: a warp copies those of four k-blocks at a time, of the tile's rows ([row][4]) and of its blocks of W ([2][4]), into a ring of
+// slots ahead of the sums (a load that a warp of the sums waits for, even one issued two k-blocks before, cost a third of the kernel's time).
+constexpr int F8_BATCH = 4, F8_SLOTS = 3, F8_SLOT = 130 * F8_BATCH * 4;
+__device__ __forceinline__ void f8_copy4(uint32_t dst, const float* src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4u : 0u) : "memory");
+}
+// k-blocks b .. b + 3: rows m0 .., blocks of W from nb on
+__device__ __forceinline__ void f8_copy_scales(uint32_t dst, uint32_t bar, const F8Scales& sc, int b, int blocks, int m0, int M, int nb, int n_blocks, int lane) {
+#pragma unroll
+    for (int k = 0; k < F8_BATCH; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = m0 + i * 32 + lane;
+            const bool live = m < M && b + k < blocks;
+            f8_copy4(dst + ((i * 32 + lane) * F8_BATCH + k) * 4, live ? sc.a + (long)(b + k) * sc.lda + m : sc.a, live);
+        }
+    if (lane < 2 * F8_BATCH) {
+        const int n = nb + lane / F8_BATCH, k = b + lane % F8_BATCH;
+        const bool live = n < n_blocks && k < blocks;
+        f8_copy4(dst + (128 * F8_BATCH + lane) * 4, live ? sc.w + (long)n * sc.ldw + k : sc.w, live);
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// all loads of tensor memory so far are in r
+__device__ __forceinline__ void f8_tmem_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+    asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                   "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+// acc += (W columns of a k-block's sums at taddr) * f; the next 32 columns are on their way while 32 are added.  read(): called when the last of
+// them has left tensor memory.
+template <int W, typename Read>
+__device__ __forceinline__ void f8_add_block(uint32_t taddr, float f, float (&acc)[W], Read read) {
+    static_assert(W % 64 == 0, "two registers' worth at a time");
+    uint32_t r0[32], r1[32];
+    tmem_ld32(taddr, r0);
+#pragma unroll
+    for (int c0 = 0; c0 < W; c0 += 64) {
+        f8_tmem_wait(r0);
+        tmem_ld32(taddr + c0 + 32, r1);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[c0 + j] = fmaf(__uint_as_float(r0[j]), f, acc[c0 + j]);
+        f8_tmem_wait(r1);
+        if (c0 + 64 < W) tmem_ld32(taddr + c0 + 64, r0);
+        else read();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[c0 + 32 + j] = fmaf(__uint_as_float(r1[j]), f, acc[c0 + 32 + j]);
+    }
+}
+
+// A warp's 32 rows x W columns of the result, a row a lane.  By TMA (the result's rows start on 16-byte borders): 128 bytes of a row at a time into
+// a buffer of 4 KB, 16-byte pieces swizzled as the copy expects them; rows and columns beyond the matrix are clipped by it.
+// Stored from registers each lane's 16 bytes are a row of their own (a tile of 128 x 256 took 6,700 cycles so).
+constexpr int F8_STORE = 4096;
+template <int W, typename TC>
+__device__ __forceinline__ void f8_store_rows(const float (&acc)[W], const CUtensorMap* map, bool by_tma, uint32_t at, TC* out, long ldc, int m, int n, int M, int N) {
+    const int lane = threadIdx.x & 31;
+    if (!by_tma) {
+        if (m + lane < M) {
+#pragma unroll
+            for (int c0 = 0; c0 < W; c0 += 32) {
+                uint32_t r[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(acc[c0 + j]);
+                if (n + c0 < N) tc_store_chunk<0, TC>(r, out, ldc, m + lane, n, c0, N);
+            }
+        }
+        return;
+    }
+    constexpr int COLS = 128 / sizeof(TC);
+#pragma unroll
+    for (int c0 = 0; c0 < W; c0 += COLS) {
+        if (lane == 0) tma_store_read<0>();                                   // the last copy has read the buffer
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            uint4 v;
+            if (sizeof(TC) == 2) {
+                uint32_t h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(acc[c0 + p * 8 + 2 * i], acc[c0 + p * 8 + 2 * i + 1]);
+                    h[i] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+                v = make_uint4(h[0], h[1], h[2], h[3]);
+            } else {
+                v = make_uint4(__float_as_uint(acc[c0 + p * 4]), __float_as_uint(acc[c0 + p * 4 + 1]), __float_as_uint(acc[c0 + p * 4 + 2]), __float_as_uint(acc[c0 + p * 4 + 3]));
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 128 + ((p ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            if (m < M && n + c0 < N) tma_store_2d(at, map, n + c0, m);
+            tma_store_commit();
+        }
+    }
+}
+
+// PAIR: two CTAs make a tile of 256 x 256 together (cta_group::2): each holds 128 rows of a and half of the tile's rows of W in its shared memory,
+// and the sums of its own rows in its tensor memory; the first issues the instructions for both.  Alone, a CTA makes 128 x 128.
+// Shared memory is what the tensor cores wait for next: per k-block of 128 x 256 sums an SM's take 64 KB out of it in a pair and 96 alone, 128 as two
+// of 128 x 128, beside the 32, 48 or 64 that TMA puts in, at 128 bytes a cycle, while the sums take 512 cycles.
+template <bool PAIR> struct F8Tiles {
+    static constexpr int P = PAIR ? 2 : 1, BM = 128 * P, BN = 128 * P;
+    static constexpr int STAGE_A = 128 * F8_KB, STAGE_W = 128 * F8_KB, STAGES = 5;
     static constexpr int BUFS = 512 / BN;
-    static constexpr int SMEM = STAGES * (STAGE_A + STAGE_W) + 1024 /*align*/ + 256 /*barriers*/;
+    static constexpr int RING = STAGES * (STAGE_A + STAGE_W), STORES = 8 * F8_STORE;
+    static constexpr int SMEM = RING + STORES + F8_SLOTS * F8_SLOT + 1024 /*align*/ + 256 /*barriers*/;
+    static_assert(SMEM <= 227 * 1024, "a CTA's shared memory");
 };
 
-// Warp 0 fetches, warp 1 multiplies, warps 2 to 9 add up: each a quarter of the tile's rows times half of its columns, a row a thread.
-template <int BN, typename TC>
-__global__ void __launch_bounds__(320, 1)
-float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, F8Scales sc, TC* __restrict__ out, long ldc,
-                    int M, int N, int K, int m_tiles, int tiles) {
-    using C = F8Tiles<BN>;
+// Rows of codes that start anywhere, which TMA does not take: 128 threads bring a tile's 128 rows x 128 codes, each 16 codes of eight rows, in aligned words that
+// are shifted into place, and put them where TMA would.  A word that reaches over an end of the row is put together from its bytes within it, so that
+// nothing outside the rows is read; codes beyond the row and rows beyond the matrix are zeros.  Twenty words of each thread are on their way at a time.
+__device__ __forceinline__ uint32_t f8_word(const uint8_t* word, const uint8_t* begin, const uint8_t* end) {
+    if (word >= begin && word + 4 <= end) return __ldcg(reinterpret_cast<const uint32_t*>(word));
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (word + i >= begin && word + i < end) v |= (uint32_t)__ldcg(word + i) << (8 * i);
+    return v;
+}
+__device__ __forceinline__ void f8_gather(uint32_t tile, const uint8_t* p, long ld, int row0, int rows, int k0, int K, int thread) {
+    const int chunk = thread & 7;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint32_t v[4][5];
+        uint32_t shift[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row0 + (thread >> 3) + (half * 4 + i) * 16;
+            const uint8_t* begin = p + (r < rows ? (long)r * ld : 0);
+            const uint8_t* end = begin + (r < rows ? K : 0);
+            const uint8_t* from = begin + k0 + chunk * 16;
+            const uint8_t* word = reinterpret_cast<const uint8_t*>((uintptr_t)from & ~(uintptr_t)3);
+            shift[i] = ((uint32_t)(uintptr_t)from & 3) * 8;
+#pragma unroll
+            for (int j = 0; j < 5; ++j) v[i][j] = f8_word(word + 4 * j, begin, end);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (thread >> 3) + (half * 4 + i) * 16;
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(v[i][j], v[i][j + 1], shift[i]);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + r * 128 + ((chunk ^ (r & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+    }
+}
+struct F8Rows {
+    const uint8_t* a;
+    long lda;
+    const uint8_t* w;
+    long ldw;
+};
+
+// Persistent.  Warp 0 fetches, warp 1 multiplies, warp 2 brings the scales, warps 4 to 11 add up: each a quarter of the tile's rows times half
+// of its columns, a row a thread; they take the registers that the first four give up.  GATHER: four more warps fetch in warp 0's place.
+template <bool PAIR, bool GATHER, typename TC>
+__global__ void __launch_bounds__(GATHER ? 512 : 384, 1)
+float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
+                    int store_by_tma, F8Scales sc, TC* __restrict__ out, long ldc, int M, int N, int K, int m_tiles, int tiles, F8Rows rows) {
+    static_assert(!(PAIR && GATHER), "rows that start anywhere are multiplied in tiles of one CTA");
+    using C = F8Tiles<PAIR>;
+    constexpr int P = C::P;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t sA = base, sW = base + C::STAGES * C::STAGE_A;
-    const uint32_t bars = base + C::STAGES * (C::STAGE_W + C::STAGE_A);
-    const uint32_t full0 = bars, empty0 = full0 + 8 * C::STAGES, tfull0 = empty0 + 8 * C::STAGES, tempty0 = tfull0 + 8 * C::BUFS, slot = tempty0 + 8 * C::BUFS;
+    const uint32_t sA = base, sW = base + C::STAGES * C::STAGE_A, sStore = base + C::RING, sScale = sStore + C::STORES;
+    const uint32_t bars = sScale + F8_SLOTS * F8_SLOT;
+    const uint32_t full0 = bars, empty0 = full0 + 8 * C::STAGES, tfull0 = empty0 + 8 * C::STAGES, tempty0 = tfull0 + 8 * C::BUFS;
+    const uint32_t sfull0 = tempty0 + 8 * C::BUFS, sempty0 = sfull0 + 8 * F8_SLOTS, slot = sempty0 + 8 * F8_SLOTS;
     volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(gen + (slot - base));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;       // (known to be the same for the whole warp)
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0, first = (int)blockIdx.x / P, step = (int)gridDim.x / P;
     const int blocks = (K + F8_KB - 1) / F8_KB;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-        for (int b = 0; b < C::BUFS; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 8); }
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full0 + 8 * s, GATHER ? 128 : 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int b = 0; b < C::BUFS; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 8 * P); }
+        for (int s = 0; s < F8_SLOTS; ++s) { mbar_init(sfull0 + 8 * s, 32); mbar_init(sempty0 + 8 * s, 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) {                                                               // both have their barriers and their columns
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *slot_ptr;
     griddep_launch();                                                         // behind the allocation: what starts now cannot take these columns and wait for this kernel
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0 && !GATHER) {
             griddep_wait();
-            int it = 0;
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                const int m0 = tile % m_tiles * 128, n0 = tile / m_tiles * BN;
-                for (int kb = 0; kb < blocks; ++kb, ++it) {
-                    const int s = it % C::STAGES, round = it / C::STAGES;
-                    if (round > 0) mbar_wait(empty0 + 8 * s, (round - 1) & 1, 1);
-                    mbar_expect_tx(full0 + 8 * s, C::STAGE_W + C::STAGE_A);
-                    tma_load_2d(sA + s * C::STAGE_A, &map_a, full0 + 8 * s, kb * F8_KB, m0);
-                    tma_load_2d(sW + s * C::STAGE_W, &map_w, full0 + 8 * s, kb * F8_KB, n0);
+            F8Ring<C::STAGES> r;
+            for (int tile = first; tile < tiles; tile += step) {
+                const int m0 = tile % m_tiles * C::BM + rank * 128, n0 = tile / m_tiles * C::BN + rank * 128;
+                for (int kb = 0; kb < blocks; ++kb, r.next()) {
+                    mbar_wait(empty0 + 8 * r.at, r.parity ^ 1, 1);            // (passes at once in the first round)
+                    if (elect_one()) {
+                        if (rank == 0) mbar_expect_tx(full0 + 8 * r.at, P * (C::STAGE_W + C::STAGE_A));
+                        if (PAIR) {                                           // both CTAs' copies arrive at the first one's barrier
+                            const uint32_t bar = tc_map_rank(full0 + 8 * r.at, 0);
+                            tma_load_2d_pair(sA + r.at * C::STAGE_A, &map_a, bar, kb * F8_KB, m0);
+                            tma_load_2d_pair(sW + r.at * C::STAGE_W, &map_w, bar, kb * F8_KB, n0);
+                        } else {
+                            tma_load_2d(sA + r.at * C::STAGE_A, &map_a, full0 + 8 * r.at, kb * F8_KB, m0);
+                            tma_load_2d(sW + r.at * C::STAGE_W, &map_w, full0 + 8 * r.at, kb * F8_KB, n0);
+                        }
+                    }
+                    __syncwarp();
                 }
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = umma_idesc_e4m3(128, BN);
-            int it = 0;
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                for (int kb = 0; kb < blocks; ++kb, ++it) {
-                    const int s = it % C::STAGES, b = it % C::BUFS, use = it / C::BUFS;
-                    mbar_wait(full0 + 8 * s, (it / C::STAGES) & 1, 2);
-                    if (use > 0) mbar_wait(tempty0 + 8 * b, (use - 1) & 1, 2);
+        } else if (warp == 1 && rank == 0) {
+            const uint32_t idesc = umma_idesc_e4m3(C::BM, C::BN);
+            const uint64_t da0 = make_desc_sw128(sA), dw0 = make_desc_sw128(sW);
+            F8Ring<C::STAGES> r;
+            F8Ring<C::BUFS> t;
+            for (int tile = first; tile < tiles; tile += step) {
+                for (int kb = 0; kb < blocks; ++kb, r.next(), t.next()) {
+                    const uint64_t da = da0 + r.at * (C::STAGE_A >> 4), dw = dw0 + r.at * (C::STAGE_W >> 4);
+                    const uint32_t d = tmem + t.at * C::BN;
+                    if (PAIR) {
+                        f8_wait_cluster(full0 + 8 * r.at, r.parity, 2);
+                        f8_wait_cluster(tempty0 + 8 * t.at, t.parity ^ 1, 2);
+                    } else {
+                        mbar_wait(full0 + 8 * r.at, r.parity, 2);
+                        mbar_wait(tempty0 + 8 * t.at, t.parity ^ 1, 2);
+                    }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t da = make_desc_sw128(sA + s * C::STAGE_A), dw = make_desc_sw128(sW + s * C::STAGE_W);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) umma_f8(tmem + b * BN, da + 2 * k, dw + 2 * k, idesc, k > 0 ? 1u : 0u);
-                    umma_commit(empty0 + 8 * s);
-                    umma_commit(tfull0 + 8 * b);
+                        for (int k = 0; k < 4; ++k) {                         // 32 codes = 2 descriptor units
+                            if (PAIR) umma_f8_pair(d, da + 2 * k, dw + 2 * k, idesc, k > 0 ? 1u : 0u);
+                            else umma_f8(d, da + 2 * k, dw + 2 * k, idesc, k > 0 ? 1u : 0u);
+                        }
+                        if (PAIR) {
+                            umma_commit_pair(tfull0 + 8 * t.at);
+                            umma_commit_pair(empty0 + 8 * r.at);
+                        } else {
+                            umma_commit(tfull0 + 8 * t.at);
+                            umma_commit(empty0 + 8 * r.at);
+                        }
+                    }
+                    __syncwarp();
                 }
+            }
+        } else if (warp == 2) {
+            griddep_wait();
+            const int n_blocks = (N + 127) / 128;
+            F8Ring<F8_SLOTS> q;
+            for (int tile = first; tile < tiles; tile += step) {
+                const int m0 = tile % m_tiles * C::BM + rank * 128, nb = tile / m_tiles * P;
+                for (int kb = 0; kb < blocks; kb += F8_BATCH, q.next()) {
+                    mbar_wait(sempty0 + 8 * q.at, q.parity ^ 1, 1);
+                    f8_copy_scales(sScale + q.at * F8_SLOT, sfull0 + 8 * q.at, sc, kb, blocks, m0, M, nb, n_blocks, lane);
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");                  // nothing on its way when the CTA leaves
+        }
+    } else if (GATHER && warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+        griddep_wait();
+        const int thread = threadIdx.x - 384;
+        F8Ring<C::STAGES> r;
+        for (int tile = first; tile < tiles; tile += step) {
+            const int m0 = tile % m_tiles * C::BM, n0 = tile / m_tiles * C::BN;
+            for (int kb = 0; kb < blocks; ++kb, r.next()) {
+                mbar_wait(empty0 + 8 * r.at, r.parity ^ 1, 1);
+                f8_gather(sA + r.at * C::STAGE_A, rows.a, rows.lda, m0, M, kb * F8_KB, K, thread);
+                f8_gather(sW + r.at * C::STAGE_W, rows.w, rows.ldw, n0, N, kb * F8_KB, K, thread);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(full0 + 8 * r.at);
             }
         }
     } else {
+        // (the shares add up to what the CTA was launched with: 40 + 2 x 232 = 3 x 168, with four warps more 40 + 120 + 2 x 176 = 4 x 128)
+        if (GATHER) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         griddep_wait();
-        constexpr int W = BN / 2;                                             // a thread's columns
-        const int quarter = warp & 3, c_first = (warp - 2) / 4 * W;
-        // the factor of the k-block after the next one is on its way: (tile, k-block) runs ahead of the sums by two
-        int ptile = blockIdx.x, pkb = 0;
-        auto fetch = [&]() {
-            float f = 0.f;
-            if (ptile < tiles) {
-                const int m = ptile % m_tiles * 128 + quarter * 32 + lane, n = ptile / m_tiles * BN + c_first;
-                if (m < M && n < N) f = __ldcg(sc.a + (long)pkb * sc.lda + m) * __ldcg(sc.w + (long)(n / 128) * sc.ldw + pkb);
-                if (++pkb == blocks) { pkb = 0; ptile += gridDim.x; }
-            }
-            return f;
-        };
-        float f1 = fetch(), f2 = fetch();
-        int it = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            uint64_t acc[W / 2];
+        constexpr int W = 64 * P;                                             // a thread's columns
+        const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
+        const uint32_t buf = sStore + (warp - 4) * F8_STORE;
+        const uint32_t columns = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * W);
+        const uint32_t factors = sScale + row * (F8_BATCH * 4), factors_w = sScale + (128 + (PAIR ? half : 0)) * (F8_BATCH * 4);
+        F8Ring<C::BUFS> t;
+        F8Ring<F8_SLOTS> q;
+        for (int tile = first; tile < tiles; tile += step) {
+            float acc[W];
 #pragma unroll
-            for (int i = 0; i < W / 2; ++i) acc[i] = 0;
-            for (int kb = 0; kb < blocks; ++kb, ++it) {
-                const float f = f1;
-                f1 = f2;
-                f2 = fetch();
-                const uint64_t s2 = f8_two(f, f);
-                const int b = it % C::BUFS;
-                mbar_wait(tfull0 + 8 * b, (it / C::BUFS) & 1, 3);
+            for (int i = 0; i < W; ++i) acc[i] = 0.f;
+            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int kb = 0; kb < blocks; ++kb, t.next()) {
+                if (kb % F8_BATCH == 0) {
+                    mbar_wait(sfull0 + 8 * q.at, q.parity, 3);
+                    const float4 fa = f8_lds4(factors + q.at * F8_SLOT), fw = f8_lds4(factors_w + q.at * F8_SLOT);
+                    f = make_float4(fa.x * fw.x, fa.y * fw.y, fa.z * fw.z, fa.w * fw.w);
+                    __syncwarp();
+                    f8_arrive0(sempty0 + 8 * q.at, lane);
+                    q.next();
+                }
+                mbar_wait(tfull0 + 8 * t.at, t.parity, 3);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                __syncwarp();
-#pragma unroll
-                for (int c0 = 0; c0 < W; c0 += 32) {
-                    uint32_t r[32];
-                    tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * BN + c_first + c0), r);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) f8_fma2(acc[c0 / 2 + j], r[2 * j], r[2 * j + 1], s2);
-                }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(tempty0 + 8 * b);
+                f8_add_block<W>(columns + t.at * C::BN, f.x, acc, [&]() {
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    const uint32_t bar = tempty0 + 8 * t.at;
+                    if (PAIR) f8_arrive0_cluster(tc_map_rank(bar, 0), lane);
+                    else f8_arrive0(bar, lane);
+                });
+                f = make_float4(f.y, f.z, f.w, 0.f);
             }
-            const int m = tile % m_tiles * 128 + quarter * 32 + lane, n0 = tile / m_tiles * BN;
-            if (m < M) {
-#pragma unroll
-                for (int c0 = 0; c0 < W; c0 += 32) {
-                    uint32_t r[32];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float2 v = f8_split(acc[c0 / 2 + j]);
-                        r[2 * j] = __float_as_uint(v.x);
-                        r[2 * j + 1] = __float_as_uint(v.y);
-                    }
-                    if (n0 + c_first + c0 < N) tc_store_chunk<0, TC>(r, out, ldc, m, n0, c_first + c0, N);
-                }
-            }
+            f8_store_rows<W, TC>(acc, &map_out, store_by_tma != 0, buf, out, ldc, tile % m_tiles * C::BM + rank * 128 + quarter * 32,
+                                 tile / m_tiles * C::BN + half * W, M, N);
         }
+        if (lane == 0) tma_store_done();
     }
+    __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) {                                                               // the first CTA's instructions read the other's shared memory, whose barriers they arrive at
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 
@@ -392,52 +688,86 @@ inline int f8_sms() {
 }
 
 template <int NT, typename TC>
-int launch_float8_few(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, cudaStream_t stream) {
+int launch_float8_few(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, int Z, int w_ready, cudaStream_t stream) {
     CUtensorMap ma, mw;
     if (!f8_make_map(&ma, a, M, K, lda, NT) || !f8_make_map(&mw, w, N, K, ldw, 128)) return AIEN_E_STATE;
-    auto kernel = float8_few_kernel<NT, TC>;
-    if (!f8_configure<float8_few_kernel<NT, TC>, F8Few<NT>::SMEM>()) return AIEN_E_STATE;
-    const long m_tiles = (M + NT - 1) / NT, n_tiles = (N + 127) / 128, blocks = (K + F8_KB - 1) / F8_KB;
+    constexpr auto kernel = float8_few_kernel<NT, TC>;
+    if (!f8_configure<kernel, F8Few<NT>::SMEM>()) return AIEN_E_STATE;
+    const long m_tiles = ((long)M + NT - 1) / NT, n_tiles = ((long)N + 127) / 128;
     if (m_tiles > 65535 || n_tiles > 65535) return AIEN_E_SHAPE;
-    int Z = 1;
-    while (Z < 8 && Z * 2 <= blocks && m_tiles * n_tiles * Z * 2 <= 2 * f8_sms()) Z *= 2;
-    return f8_launch(kernel, dim3(Z, (unsigned)m_tiles, (unsigned)n_tiles), 192, F8Few<NT>::SMEM, Z, stream, ma, mw, sc, (TC*)out, ldc, M, N, K);
+    return f8_launch(kernel, dim3(Z, (unsigned)m_tiles, (unsigned)n_tiles), 192, F8Few<NT>::SMEM, Z, stream, ma, mw, sc, (TC*)out, ldc, M, N, K, w_ready);
 }
 
-template <int BN, typename TC>
+template <bool PAIR, bool GATHER, typename TC>
 int launch_float8_tiles(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, cudaStream_t stream) {
-    CUtensorMap ma, mw;
-    if (!f8_make_map(&ma, a, M, K, lda, 128) || !f8_make_map(&mw, w, N, K, ldw, BN)) return AIEN_E_STATE;
-    auto kernel = float8_tiles_kernel<BN, TC>;
-    if (!f8_configure<float8_tiles_kernel<BN, TC>, F8Tiles<BN>::SMEM>()) return AIEN_E_STATE;
-    const long m_tiles = (M + 127) / 128, tiles = m_tiles * ((N + BN - 1) / BN);
-    if (tiles * ((K + F8_KB - 1) / F8_KB) > 2147483647L) return AIEN_E_SHAPE;
-    const int ctas = (int)(tiles < f8_sms() ? tiles : f8_sms());
-    return f8_launch(kernel, dim3(ctas), 320, F8Tiles<BN>::SMEM, 1, stream, ma, mw, sc, (TC*)out, ldc, M, N, K, (int)m_tiles, (int)tiles);
+    using C = F8Tiles<PAIR>;
+    constexpr int P = C::P;
+    CUtensorMap ma = {}, mw = {}, mo = {};
+    if (!GATHER && (!f8_make_map(&ma, a, M, K, lda, 128) || !f8_make_map(&mw, w, N, K, ldw, 128))) return AIEN_E_STATE;
+    const bool by_tma = ((uintptr_t)out & 15) == 0 && (M == 1 || ldc * sizeof(TC) % 16 == 0);
+    if (by_tma && !f8_make_map_out<TC>(&mo, out, M, N, ldc)) return AIEN_E_STATE;
+    constexpr auto kernel = float8_tiles_kernel<PAIR, GATHER, TC>;
+    if (!f8_configure<kernel, C::SMEM>()) return AIEN_E_STATE;
+    const long m_tiles = ((long)M + C::BM - 1) / C::BM, tiles = m_tiles * (((long)N + C::BN - 1) / C::BN);
+    if (tiles > 2147483647L) return AIEN_E_SHAPE;
+    const long at_once = f8_sms() / P;
+    return f8_launch(kernel, dim3((unsigned)((tiles < at_once ? tiles : at_once) * P)), GATHER ? 512 : 384, C::SMEM, P, stream, ma, mw, mo, (int)by_tma, sc,
+                     (TC*)out, ldc, M, N, K, (int)m_tiles, (int)tiles, F8Rows{(const uint8_t*)a, lda, (const uint8_t*)w, ldw});
+}
+
+// The product's form, by the time that each would take (us; measured with K of 4,096 and 12,288 on rows of 8 to 4,096, with one to three waves):
+//   in tiles of 128 x 128      3.2 and 0.28 a k-block and wave of one tile an SM
+//   in pairs, 256 x 256        3.0 and 0.44 a k-block and wave of one tile a pair of SMs
+//   few rows, 128 x NT         2.3, shared by a cluster 4.0, and a k-block 0.23 where the CTAs are few, else W's bytes at 6.5 TB/s; with 64
+//                              columns 0.0016 a CTA, which L2 and the reading of tensor memory take; two CTAs an SM
+// 256 x 4,096 x 4,096: 11.8 us in tiles, 15.5 in pairs, 16.6 in the form for few rows; 128 x 4,096 x 12,288: 28.2, 37.0 and 18.2;
+// 1,024 x 4,096 x 4,096: 20.7, 17.1 and 36.8.
+struct F8Plan {
+    int form, Z;              // columns of the form for few rows (16, 32 or 64), 1 tiles, 2 pairs; CTAs that share K
+};
+inline F8Plan f8_plan(int M, int N, int K) {
+    const long sms = f8_sms(), blocks = ((long)K + F8_KB - 1) / F8_KB, n_tiles = ((long)N + 127) / 128;
+    const int nt = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    const long few = ((long)M + nt - 1) / nt * n_tiles;
+    F8Plan best = {nt, 1};
+    double least = 1e30;
+    for (int Z = 1; Z <= 8 && Z <= blocks; Z *= 2) {
+        const long ctas = few * Z, at_once = ctas < 2 * sms ? ctas : 2 * sms;
+        const double busy = at_once * (nt == 64 ? 0.0016 + (M <= 64 ? 0.0009 : 0.) : 0.0025), each = busy > 0.23 ? busy : 0.23;
+        const double t = (Z == 1 ? 2.3 : 4.0) + (double)((blocks + Z - 1) / Z) * each * (double)((ctas + 2 * sms - 1) / (2 * sms));
+        if (t < least) { least = t; best.Z = Z; }
+    }
+    if (M <= 64) return best;
+    const long alone = ((long)M + 127) / 128 * n_tiles, pairs = ((long)M + 255) / 256 * (((long)N + 255) / 256);
+    const double t1 = 3.2 + 0.28 * blocks * (double)((alone + sms - 1) / sms), t2 = 3.0 + 0.44 * blocks * (double)((pairs + sms / 2 - 1) / (sms / 2));
+    if (least <= t1 && least <= t2) return best;
+    return t1 <= t2 ? F8Plan{1, 1} : F8Plan{2, 1};
 }
 
 template <typename TC>
-int launch_float8(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, cudaStream_t stream) {
-#define F8_FEW(NT) return launch_float8_few<NT, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream)
-#define F8_TILES(BN) return launch_float8_tiles<BN, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream)
-    if (M <= 16) F8_FEW(16);
-    if (M <= 32) F8_FEW(32);
-    if (M <= 256) F8_FEW(64);
-    if (((long)(M + 127) / 128) * ((N + 255) / 256) >= f8_sms()) F8_TILES(256);
-    F8_TILES(128);
+int launch_float8(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, int w_ready, cudaStream_t stream) {
+    const bool whole = (((uintptr_t)a | (uintptr_t)w) & 15) == 0 && (M == 1 || lda % 16 == 0) && (N == 1 || ldw % 16 == 0);
+    if (!whole) return launch_float8_tiles<false, true, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream);
+    const F8Plan plan = f8_plan(M, N, K);
+#define F8_FEW(NT) return launch_float8_few<NT, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, plan.Z, w_ready, stream)
+    if (plan.form == 16) F8_FEW(16);
+    if (plan.form == 32) F8_FEW(32);
+    if (plan.form == 64) F8_FEW(64);
 #undef F8_FEW
-#undef F8_TILES
+    if (plan.form == 1) return launch_float8_tiles<false, false, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream);
+    return launch_float8_tiles<true, false, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream);
 }
 
 }  // namespace aien
 
-// Whether the tensor-core forms take codes that lie like this: every row on a 16-byte border.
-AIEN_API int aien_matmul_float8_tc(const void* a, long lda, const float* sa, long lds, const void* w, long ldw, const float* sw, long ldsw,
-                                   void* out, int c_dt, long ldc, int M, int N, int K, cudaStream_t stream) {
+// a [M, K] and w [N, K] codes, rows lda and ldw bytes apart; sa [ceil(K / 128), M] (lds numbers apart); sw [ceil(N / 128), ceil(K / 128)] (ldsw
+// numbers apart); out [M, N], rows ldc numbers apart.  w_ready: w and its scales were written by nothing that an unfinished kernel ahead in the stream
+// does, so that they may be requested before it is done.
+AIEN_API int aien_matmul_float8(const void* a, long lda, const float* sa, long lds, const void* w, long ldw, const float* sw, long ldsw,
+                                   void* out, int c_dt, long ldc, int M, int N, int K, int w_ready, cudaStream_t stream) {
     using namespace aien;
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) return AIEN_E_SHAPE;
-    if (((uintptr_t)a & 15) || ((uintptr_t)w & 15) || (M > 1 && (lda & 15)) || (N > 1 && (ldw & 15))) return AIEN_E_ALIGN;
     const F8Scales sc{sa, lds, sw, ldsw};
-    AIEN_DISPATCH_DTYPE(c_dt, TC, return (launch_float8<TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream)));
+    AIEN_DISPATCH_DTYPE(c_dt, TC, return (launch_float8<TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, w_ready, stream)));
 }

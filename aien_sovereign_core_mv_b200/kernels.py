@@ -2574,9 +2574,12 @@ def quantize_blocks_float8(w: torch.Tensor, codes: torch.Tensor, scales: torch.T
     _check(lib().aien_quantize_blocks_float8(w, dt(w), _ld(w), codes, _ld(codes), scales, _ld(scales), N, width, _stream()), name)
 
 
-def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> None:
+def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, w_ready: bool = False) -> None:
     """out [M, N] (bfloat16 or float32, row stride free) = a . w^T of rows a [M, K] with scales [ceil(K / 128), M] and a weight w [N, K] with scales
-    [ceil(N / 128), ceil(K / 128)]: a block's sum of code products times its two scales, the blocks added up in float32."""
+    [ceil(N / 128), ceil(K / 128)]: a block's sum of code products times its two scales, the blocks added up in float32.
+
+    ``w_ready``: w was written before the kernels that are unfinished in the stream were launched (a model's weights during a step), so that
+    it may be requested ahead of their end."""
     name = "matmul_float8"
     M, N = out.shape
     width = a.shape[-1]
@@ -2589,4 +2592,4 @@ def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_sc
     _rows_of(name, "out", out, (M, N), _F32_BF16)
     _here(name, a, a_scales, w, w_scales, out)
     _check(lib().aien_matmul_float8(a, _ld(a), a_scales, _ld(a_scales), w, _ld(w), w_scales, _ld(w_scales), out, dt(out), _ld(out), M, N, width,
-                                    _stream()), name)
+                                    1 if w_ready else 0, _stream()), name)
