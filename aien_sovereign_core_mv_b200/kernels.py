@@ -175,8 +175,13 @@ class stream_scope:
         return False
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # the current stream's handle without an object around it: 0.2 us for 1.0
+
+
 def _stream() -> int:
-    return _STREAM if _STREAM is not None else torch.cuda.current_stream().cuda_stream
+    if _STREAM is not None:
+        return _STREAM
+    return _raw_stream(torch.cuda.current_device()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 def dt(t: torch.Tensor) -> int:
@@ -2481,6 +2486,22 @@ def _rows_of(name: str, what: str, t: torch.Tensor, shape: tuple, dtypes: tuple)
         _refuse(name, f"{what} has strides {tuple(t.stride())}: its rows must be whole and apart")
 
 
+def _two(name: str, t: torch.Tensor) -> tuple:
+    """(rows, columns) of a matrix with columns."""
+    if t.dim() != 2:
+        _refuse(name, f"a matrix is wanted, not {t.dim()} dimensions")
+    rows, cols = t.shape
+    if cols < 1:
+        _refuse(name, "rows of no numbers")
+    return rows, cols
+
+
+def _whole(name: str, what: str, t: torch.Tensor) -> torch.Tensor:
+    if not t.is_contiguous():
+        _refuse(name, f"{what} must be contiguous")
+    return t
+
+
 def _here(name: str, *ts: Optional[torch.Tensor]) -> None:
     """Every tensor lives on the device that the launch goes to."""
     for t in ts:
@@ -2497,81 +2518,87 @@ _F32 = (torch.float32,)
 _F32_BF16 = (torch.float32, torch.bfloat16)
 
 
-def _float8_result(name: str, codes: torch.Tensor, scales: torch.Tensor, T: int, width: int) -> None:
-    if width < 1:
-        _refuse(name, "rows of no numbers")
-    _rows_of(name, "codes", codes, (T, width), _E4M3)
-    _rows_of(name, "scales", scales, (float8_blocks(width), T), _F32)
+def _matrix(t: torch.Tensor, rows: int, cols: int, types: int) -> int:
+    """Numbers between the rows of a matrix of this size on the current device, of a type in ``types``; -1 where it is not that (the native check takes this one's place)."""
+    global _matrix
+    _matrix = _build.load_launch().matrix
+    return _matrix(t, rows, cols, types)
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Numbers between a matrix's rows; of a single row, its length."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _explain(name: str, *wanted) -> None:
+    """Raises what is wrong with the first of (what, tensor, shape, dtypes) that is not as wanted, or with where one of them lives."""
+    for what, t, shape, dtypes in wanted:
+        _rows_of(name, what, t, shape, dtypes)
+    _here(name, *(t for _, t, _, _ in wanted))
+    _refuse(name, "an argument is not what it should be")
 
 
 def quantize_rows_float8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
     """x [T, K] float32 or bfloat16 (row stride free) in 8 bits: codes [T, K] e4m3, scales [ceil(K / 128), T] float32."""
-    T, width = codes.shape
-    _rows_of("quantize_rows_float8", "x", x, (T, width), _F32_BF16)
-    _float8_result("quantize_rows_float8", codes, scales, T, width)
-    _here("quantize_rows_float8", x, codes, scales)
-    _check(lib().aien_quantize_rows_float8(x, dt(x), _ld(x), codes, _ld(codes), scales, _ld(scales), T, width, _stream()), "quantize_rows_float8")
+    name = "quantize_rows_float8"
+    T, width = _two(name, codes)
+    blocks = float8_blocks(width)
+    ldx, ldc, lds = _matrix(x, T, width, 3), _matrix(codes, T, width, 4), _matrix(scales, blocks, T, 1)
+    if ldx < 0 or ldc < 0 or lds < 0:
+        _explain(name, ("x", x, (T, width), _F32_BF16), ("codes", codes, (T, width), _E4M3), ("scales", scales, (blocks, T), _F32))
+    _check(lib().aien_quantize_rows_float8(x, dt(x), ldx, codes, ldc, scales, lds, T, width, _stream()), name)
 
 
 def swiglu_float8(gate_up: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: int = 0, act: str = "silu") -> None:
     """:func:`swiglu` with its result in 8 bits: act(gate) * up of gate_up [T, 2K], float32 or bfloat16, contiguous, computed in float32,
     as codes [T, K] and scales [ceil(K / 128), T]."""
-    T, width = codes.shape
     name = "swiglu_float8"
+    T, width = _two(name, codes)
+    blocks = float8_blocks(width)
     if act not in GATED_ACTS:
         _refuse(name, f"activation {act!r}: known are {sorted(GATED_ACTS)}")
     if group < 0 or (group > 0 and width % group):
         _refuse(name, f"{width} columns do not divide into runs of {group}")
-    if not gate_up.is_contiguous():
-        _refuse(name, "gate_up must be contiguous")
-    _rows_of(name, "gate_up", gate_up, (T, 2 * width), _F32_BF16)
-    _float8_result(name, codes, scales, T, width)
-    _here(name, gate_up, codes, scales)
-    _check(lib().aien_swiglu_float8(gate_up, dt(gate_up), int(group), 1 if act == "gelu_tanh" else 0, codes, _ld(codes), scales, _ld(scales), T, width,
-                                    _stream()), name)
+    ldg, ldc, lds = _matrix(gate_up, T, 2 * width, 3 + 8), _matrix(codes, T, width, 4), _matrix(scales, blocks, T, 1)
+    if ldg < 0 or ldc < 0 or lds < 0:
+        _explain(name, ("gate_up", _whole(name, "gate_up", gate_up), (T, 2 * width), _F32_BF16), ("codes", codes, (T, width), _E4M3),
+                 ("scales", scales, (blocks, T), _F32))
+    _check(lib().aien_swiglu_float8(gate_up, dt(gate_up), int(group), 1 if act == "gelu_tanh" else 0, codes, ldc, scales, lds, T, width, _stream()), name)
 
 
 def add_rmsnorm_float8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float, codes: torch.Tensor, scales: torch.Tensor) -> None:
     """:func:`add_rmsnorm` with its result in 8 bits: x [T, H] float32 += delta (when given: [T, H] in any kernel dtype, or float32 partial
     products [P, T, H]) in place; rmsnorm(x) * weight as codes [T, H] and scales [ceil(H / 128), T]."""
-    T, H = codes.shape
     name = "add_rmsnorm_float8"
-    if not x.is_contiguous():
-        _refuse(name, "x must be contiguous")
-    _rows_of(name, "x", x, (T, H), _F32)
+    T, H = _two(name, codes)
+    blocks = float8_blocks(H)
+    ldx, ldc, lds = _matrix(x, T, H, 1 + 8), _matrix(codes, T, H, 4), _matrix(scales, blocks, T, 1)
     nparts, stride = 1, 0
     if delta is not None:
-        if delta.dim() == 3 and delta.dtype == torch.float32 and delta.shape[0] >= 1 and delta.is_contiguous():
-            nparts, stride = delta.shape[0], T * H
-            _rows_of(name, "delta", delta.view(nparts * T, H), (nparts * T, H), _F32)
-        else:
-            if not delta.is_contiguous():
-                _refuse(name, "delta must be contiguous")
-            _rows_of(name, "delta", delta, (T, H), _F32_BF16)
-    if weight.numel() != H or not weight.is_contiguous() or weight.dtype not in _F32_BF16:
+        if delta.dim() == 3:
+            nparts, stride = _matrix(delta, T, H, 1 + 8 + 16), T * H
+        elif _matrix(delta, T, H, 3 + 8) < 0:
+            nparts = -1
+    if weight.dim() != 1 or weight.numel() != H or not weight.is_contiguous() or weight.dtype not in _F32_BF16:
         _refuse(name, f"weight must be {H} contiguous numbers, float32 or bfloat16")
-    _float8_result(name, codes, scales, T, H)
-    _here(name, x, delta, weight, codes, scales)
-    _check(lib().aien_add_rmsnorm_float8(x, delta, dt(delta) if delta is not None else F32, nparts, stride, weight, dt(weight), float(eps),
-                                         codes, _ld(codes), scales, _ld(scales), T, H, _stream()), name)
+    if ldx < 0 or ldc < 0 or lds < 0 or nparts < 1 or weight.get_device() != x.get_device():
+        wanted = [("x", _whole(name, "x", x), (T, H), _F32), ("codes", codes, (T, H), _E4M3), ("scales", scales, (blocks, T), _F32)]
+        if delta is not None and delta.dim() == 3:
+            P = delta.shape[0]
+            if P < 1 or tuple(delta.shape[1:]) != (T, H):
+                _refuse(name, f"delta has shape {tuple(delta.shape)}, not parts of {(T, H)}")
+            wanted.append(("delta", _whole(name, "delta", delta).view(P * T, H), (P * T, H), _F32))
+        elif delta is not None:
+            wanted.append(("delta", _whole(name, "delta", delta), (T, H), _F32_BF16))
+        _explain(name, *wanted)
+    _check(lib().aien_add_rmsnorm_float8(x, delta, F32 if delta is None else dt(delta), nparts, stride, weight, dt(weight), float(eps),
+                                         codes, ldc, scales, lds, T, H, _stream()), name)
 
 
 def quantize_blocks_float8(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
     """A weight w [N, K] float32 or bfloat16 (row stride free) in 8 bits: codes [N, K] e4m3, scales [ceil(N / 128), ceil(K / 128)] float32."""
-    N, width = codes.shape
     name = "quantize_blocks_float8"
-    if width < 1:
-        _refuse(name, "rows of no numbers")
-    _rows_of(name, "w", w, (N, width), _F32_BF16)
-    _rows_of(name, "codes", codes, (N, width), _E4M3)
-    _rows_of(name, "scales", scales, (float8_blocks(N), float8_blocks(width)), _F32)
-    _here(name, w, codes, scales)
-    _check(lib().aien_quantize_blocks_float8(w, dt(w), _ld(w), codes, _ld(codes), scales, _ld(scales), N, width, _stream()), name)
+    N, width = _two(name, codes)
+    shape = (float8_blocks(N), float8_blocks(width))
+    ldw, ldc, lds = _matrix(w, N, width, 3), _matrix(codes, N, width, 4), _matrix(scales, shape[0], shape[1], 1)
+    if ldw < 0 or ldc < 0 or lds < 0:
+        _explain(name, ("w", w, (N, width), _F32_BF16), ("codes", codes, (N, width), _E4M3), ("scales", scales, shape, _F32))
+    _check(lib().aien_quantize_blocks_float8(w, dt(w), ldw, codes, ldc, scales, lds, N, width, _stream()), name)
 
 
 def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, w_ready: bool = False) -> None:
@@ -2581,15 +2608,14 @@ def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_sc
     ``w_ready``: w was written before the kernels that are unfinished in the stream were launched (a model's weights during a step), so that
     it may be requested ahead of their end."""
     name = "matmul_float8"
+    width = _two(name, a)[1]
+    if out.dim() != 2:
+        _refuse(name, f"a matrix is wanted, not {out.dim()} dimensions")
     M, N = out.shape
-    width = a.shape[-1]
-    if width < 1:
-        _refuse(name, "rows of no numbers")
-    _rows_of(name, "a", a, (M, width), _E4M3)
-    _rows_of(name, "a_scales", a_scales, (float8_blocks(width), M), _F32)
-    _rows_of(name, "w", w, (N, width), _E4M3)
-    _rows_of(name, "w_scales", w_scales, (float8_blocks(N), float8_blocks(width)), _F32)
-    _rows_of(name, "out", out, (M, N), _F32_BF16)
-    _here(name, a, a_scales, w, w_scales, out)
-    _check(lib().aien_matmul_float8(a, _ld(a), a_scales, _ld(a_scales), w, _ld(w), w_scales, _ld(w_scales), out, dt(out), _ld(out), M, N, width,
-                                    1 if w_ready else 0, _stream()), name)
+    blocks, n_blocks = float8_blocks(width), float8_blocks(N)
+    lda, ldsa, ldw = _matrix(a, M, width, 4), _matrix(a_scales, blocks, M, 1), _matrix(w, N, width, 4)
+    ldsw, ldo = _matrix(w_scales, n_blocks, blocks, 1), _matrix(out, M, N, 3)
+    if lda < 0 or ldsa < 0 or ldw < 0 or ldsw < 0 or ldo < 0:
+        _explain(name, ("out", out, (M, N), _F32_BF16), ("a", a, (M, width), _E4M3), ("a_scales", a_scales, (blocks, M), _F32), ("w", w, (N, width), _E4M3),
+                 ("w_scales", w_scales, (n_blocks, blocks), _F32))
+    _check(lib().aien_matmul_float8(a, lda, a_scales, ldsa, w, ldw, w_scales, ldsw, out, dt(out), ldo, M, N, width, 1 if w_ready else 0, _stream()), name)
