@@ -30,6 +30,8 @@ def _ids(text: str):
 def _engine_args(ap):
     ap.add_argument("--model-dir", default=os.environ.get("AIEN_MODEL_DIR"), help="folder with config.json and model.safetensors")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default="stored", choices=["stored", "float8"],
+                    help="float8: the layers' matrices in 8 bits with a scale for each block of 128 (bfloat16, Llama and Qwen3 decoders)")
     ap.add_argument("--max-context", type=int, default=int(os.environ.get("AIEN_KV_CONTEXT_TOKENS", "0")),
                     help="longest request in tokens (0: the model's max_position_embeddings)")
     ap.add_argument("--batch-slots", type=int, default=64, help="requests live at a time")
@@ -48,7 +50,7 @@ def _build_engine(args):
     raw = read_config_json(args.model_dir)
     ctx = args.max_context or int(raw.get("max_position_embeddings", 4096))
     pages = args.num_pages or min(args.batch_slots * ((ctx + args.page_size - 1) // args.page_size), (1 << 20))
-    ec = EngineConfig(dtype=args.dtype, page_size=args.page_size, num_pages=pages, max_requests=args.batch_slots,
+    ec = EngineConfig(dtype=args.dtype, weights=args.weights, page_size=args.page_size, num_pages=pages, max_requests=args.batch_slots,
                       max_context=ctx, max_batch_tokens=args.max_batch_tokens, max_batch_size=args.batch_slots,
                       max_prefill_tokens=min(args.max_batch_tokens, 2048), prefill_chunk_size=args.prefill_chunk_size)
     return Engine.from_folder(args.model_dir, ec, strict=args.strict_config)

@@ -30,6 +30,14 @@ class EngineConfig:
     async_scheduling: bool = True      # plan and launch step n+1 while step n runs; its tokens are fed on the device
     replay_steps: bool = True          # a step shaped like an earlier one re-issues that step's launches as recorded
     seed: int = 0
+    weights: str = "stored"            # "stored": a layer's matrices as the checkpoint has them; "float8": in 8 bits, a scale for each 128 x 128 (bfloat16 only)
+
+    def resolved_weights(self) -> str:
+        if self.weights not in ("stored", "float8"):
+            raise ValueError(f"weights must be stored or float8, got {self.weights!r}")
+        if self.weights == "float8" and self.resolved_dtype() != "bfloat16":
+            raise ValueError("weights float8 belong to a bfloat16 engine: a float32 engine multiplies in 32 bits")
+        return self.weights
 
     def resolved_dtype(self) -> str:
         d = {"bf16": "bfloat16", "bfloat16": "bfloat16", "fp32": "float32", "float32": "float32"}.get(self.dtype)

@@ -139,14 +139,14 @@ class Engine:
     @classmethod
     def from_folder(cls, model_dir: str, engine_config: Optional[EngineConfig] = None, strict: bool = False) -> "Engine":
         ec = engine_config or EngineConfig()
-        cfg, model = build_model_from_folder(model_dir, ec.resolved_dtype(), strict)
+        cfg, model = build_model_from_folder(model_dir, ec.resolved_dtype(), strict, ec.resolved_weights())
         return cls(model, cfg, ec)
 
     @classmethod
     def from_config(cls, raw_config: Mapping, seed: int = 0, engine_config: Optional[EngineConfig] = None,
                     init_std: Optional[float] = None, device_init: bool = False) -> "Engine":
         ec = engine_config or EngineConfig()
-        cfg, model = build_model_from_config(raw_config, seed, ec.resolved_dtype(), init_std, device_init)
+        cfg, model = build_model_from_config(raw_config, seed, ec.resolved_dtype(), init_std, device_init, ec.resolved_weights())
         return cls(model, cfg, ec)
 
     # ------------------------------------------------------------------ metadata layout

@@ -9,6 +9,7 @@ from ..registry import get_architecture
 from ..weights.loader import iter_checkpoint
 from ..weights.random_init import random_tensors, write_model_folder
 from .decoder import Decoder
+from .float8 import with_float8_weights
 
 
 def model_spec_for(raw_config: Mapping, generation_config: Optional[Mapping] = None, strict: bool = False):
@@ -25,22 +26,23 @@ def model_spec_for(raw_config: Mapping, generation_config: Optional[Mapping] = N
     return builder(raw_config, generation_config, strict)
 
 
-def build_model_from_folder(model_dir: str, dtype: str, strict: bool = False) -> Tuple[object, Decoder]:
+def build_model_from_folder(model_dir: str, dtype: str, strict: bool = False, weights: str = "stored") -> Tuple[object, Decoder]:
+    """``weights`` "float8": the layers' matrices are taken to 8 bits as they are bound (``models/float8.py``)."""
     raw = read_config_json(model_dir)
     cfg, spec = model_spec_for(raw, read_generation_config(model_dir), strict)
-    model = Decoder(spec)
+    model = Decoder(with_float8_weights(spec) if weights == "float8" else spec)
     shapes = {name: shape for name, (shape, _) in model.catalog().items()}
     model.bind(iter_checkpoint(model_dir, shapes, dtype, strict))
     return cfg, model
 
 
 def build_model_from_config(raw_config: Mapping, seed: int, dtype: str, init_std: Optional[float] = None,
-                            device_init: bool = False) -> Tuple[object, Decoder]:
+                            device_init: bool = False, weights: str = "stored") -> Tuple[object, Decoder]:
     """Random weights without a folder.  ``device_init`` draws on the GPU (fast for large
-    models; the values differ from the host generator's but depend on the seed alone)."""
+    models; the values differ from the host generator's but depend on the seed alone).  ``weights`` as for a folder."""
     import torch
     cfg, spec = model_spec_for(raw_config)
-    model = Decoder(spec)
+    model = Decoder(with_float8_weights(spec) if weights == "float8" else spec)
 
     def gen():
         for name, t in random_tensors(model.catalog(), seed, init_std, "cuda" if device_init else "cpu"):

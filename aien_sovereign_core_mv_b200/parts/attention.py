@@ -8,8 +8,8 @@ import torch
 
 from .. import kernels as K
 from ..registry import register_mixer
-from .base import CacheNeed, Mixer, Position, Prenormed, ResidualSink, RunBinding, StepContext
-from .linear import linear, linear_into_residual, linear_prenormed
+from .base import CacheNeed, Float8Rows, Mixer, Position, Prenormed, ResidualSink, RunBinding, StepContext
+from .linear import Float8Matrix, float8_rows, linear, linear_float8, linear_into_residual, linear_prenormed
 
 
 @register_mixer("paged_attention")
@@ -21,10 +21,15 @@ class PagedAttention(Mixer):
     src/backend.rs:311-379; the stacked q|k|v rows follow src/resident.rs:284-288.
 
     A run that does not write its cache (``run.writes == False``) projects q only and attends
-    over the planes another run filled."""
+    over the planes another run filled.
+
+    ``weights`` "float8": h comes in 8 bits, the matrices are kept and multiplied in 8 bits, the attention's output is taken to 8 bits for the
+    last one."""
+
+    offers_float8 = True
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int, position: Position,
-                 qk_norm: bool = False, qk_norm_eps: float = 1e-6, window: int = 0, scale: Optional[float] = None):
+                 qk_norm: bool = False, qk_norm_eps: float = 1e-6, window: int = 0, scale: Optional[float] = None, weights: str = "stored"):
         if num_heads % num_kv_heads:
             raise ValueError(f"num_heads {num_heads} is not a multiple of num_kv_heads {num_kv_heads}")
         if head_dim % 2 or head_dim > 256:
@@ -37,6 +42,10 @@ class PagedAttention(Mixer):
         self.window = int(window or 0)
         self.scale = float(scale) if scale is not None else 1.0 / math.sqrt(head_dim)
         self.q_dim, self.kv_dim = self.num_heads * self.head_dim, self.num_kv_heads * self.head_dim
+        if weights not in ("stored", "float8"):
+            raise ValueError(f"weights {weights!r}: known are 'stored' and 'float8'")
+        if weights == "float8":
+            self.takes_float8, self.takes_prenormed, self.feeds_residual = True, False, False
         self.w_qkv = self.w_o = self.q_norm_w = self.k_norm_w = None
 
     # ---- tensors
@@ -57,6 +66,8 @@ class PagedAttention(Mixer):
             q, k, v = q.float(), k.float(), v.float()
         self.w_qkv = torch.cat([q, k, v], dim=0).contiguous()       # rows q | k | v
         self.w_o = tensors["o_proj"].contiguous()
+        if self.takes_float8:
+            self.w_qkv, self.w_o = Float8Matrix.of(self.w_qkv), Float8Matrix.of(self.w_o)
         if self.qk_norm:
             qn, kn = tensors["q_norm"], tensors["k_norm"]
             if qn.dtype != kn.dtype:
@@ -69,19 +80,27 @@ class PagedAttention(Mixer):
     def workspace_bytes(self, lim):
         return lim.max_tokens * (2 * self.q_dim + 2 * self.kv_dim + self.q_dim + self.hidden_size) * lim.itemsize + 4096 \
             + 8 * K.GEMV_MAX_ROWS * (self.q_dim + 2 * self.kv_dim + self.hidden_size) * 4 + 2 * K.PARTIALS_MAX_BYTES \
-            + K.attention_workspace_bytes(lim, self.num_heads, self.head_dim) + K.FUSED_NORM_SCRATCH_BYTES(self.hidden_size)
+            + K.attention_workspace_bytes(lim, self.num_heads, self.head_dim) + K.FUSED_NORM_SCRATCH_BYTES(self.hidden_size) \
+            + (Float8Rows.workspace_bytes(lim, self.hidden_size) + Float8Rows.workspace_bytes(lim, self.q_dim) if self.takes_float8 else 0)
 
     # ---- one step
     takes_prenormed = True
     feeds_residual = True
 
-    def _project(self, ctx: StepContext, h, w: torch.Tensor) -> torch.Tensor:
+    def _project(self, ctx: StepContext, h, w) -> torch.Tensor:
+        if self.takes_float8:
+            return linear_float8(ctx, h, w)
         if isinstance(h, Prenormed):
             y = linear_prenormed(ctx, h, w)
             if y is not None:
                 return y
             h = h.materialise(ctx)
         return linear(ctx, h, w, may_defer_sum=True)
+
+    def _output(self, ctx: StepContext, out: torch.Tensor, sink: Optional[ResidualSink] = None):
+        if self.takes_float8:
+            return linear_float8(ctx, float8_rows(ctx, out), self.w_o)
+        return linear_into_residual(ctx, out, self.w_o, sink) or linear(ctx, out, self.w_o, may_defer_sum=True)
 
     def forward(self, ctx: StepContext, h, run: RunBinding, sink: Optional[ResidualSink] = None):
         T = ctx.num_tokens
@@ -91,7 +110,7 @@ class PagedAttention(Mixer):
             qkv = self._project(ctx, h, self.w_qkv)
             q, k, v = qkv[..., :self.q_dim], qkv[..., self.q_dim:self.q_dim + self.kv_dim], qkv[..., self.q_dim + self.kv_dim:]
         else:
-            q = self._project(ctx, h, self.w_qkv[:self.q_dim])
+            q = self._project(ctx, h, self.w_qkv.first_rows(self.q_dim) if self.takes_float8 else self.w_qkv[:self.q_dim])
             k = v = None
         rot = self.position.rotary(ctx)
         cos, sin, rdim = rot if rot is not None else (None, None, 0)
@@ -104,7 +123,7 @@ class PagedAttention(Mixer):
             K.paged_attention_decode_fused(ctx, q, k, v, self.q_norm_w, self.k_norm_w, self.qk_norm_eps, cos, sin, rdim, group,
                                            k_cache, v_cache, out, self.num_heads, self.num_kv_heads, self.head_dim,
                                            self.window, self.scale)
-            return linear(ctx, out, self.w_o, may_defer_sum=True)
+            return self._output(ctx, out)
         q_out = ctx.workspace.take((T, self.q_dim), ctx.dtype) if q.dim() == 3 else q
         K.qk_norm_rope_kv_write(q, k, v, self.head_dim, self.q_norm_w, self.k_norm_w if k is not None else None,
                                 self.qk_norm_eps, cos, sin, rdim,
@@ -115,7 +134,7 @@ class PagedAttention(Mixer):
         out = ctx.workspace.take((T, self.q_dim), ctx.dtype)
         K.paged_attention(ctx, q_out, k_cache, v_cache, group, out, self.num_heads, self.num_kv_heads, self.head_dim,
                           self.window, self.scale)
-        return linear_into_residual(ctx, out, self.w_o, sink) or linear(ctx, out, self.w_o, may_defer_sum=True)
+        return self._output(ctx, out, sink)
 
 
 from .state_space import BranchMixer            # noqa: E402  (the two-products form this mixer follows)

@@ -142,7 +142,8 @@ class StepLimits:
     itemsize: int          # bytes of the compute dtype
 
 
-_ELEMENT_SIZE = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2, torch.int32: 4, torch.int64: 8, torch.uint8: 1, torch.float64: 8}
+_ELEMENT_SIZE = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2, torch.int32: 4, torch.int64: 8, torch.uint8: 1, torch.float64: 8,
+                 torch.float8_e4m3fn: 1}
 
 
 _LAYOUTS: Dict[tuple, Tuple[int, tuple]] = {}          # shape -> (numbers, strides), of the shapes asked for lately
@@ -244,6 +245,26 @@ class Prenormed:
 
 
 @dataclass
+class Float8Rows:
+    """Rows in 8 bits: e4m3 codes [T, K] and a float32 scale for each 128 numbers of a row, [ceil(K / 128), T] (``kernels.quantize_rows_float8``).  What
+    a part with ``takes_float8`` reads."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @staticmethod
+    def take(ctx: "StepContext", T: int, width: int) -> "Float8Rows":
+        """Room for them from the layer workspace, every row on a 16-byte border."""
+        ld = (width + 15) // 16 * 16
+        codes = ctx.workspace.take((T, ld), torch.float8_e4m3fn)
+        return Float8Rows(codes if ld == width else codes[:, :width], ctx.workspace.take(((width + 127) // 128, T), torch.float32))
+
+    @staticmethod
+    def workspace_bytes(lim: "StepLimits", width: int) -> int:
+        return lim.max_tokens * ((width + 15) // 16 * 16 + 4 * ((width + 127) // 128)) + 512
+
+
+@dataclass
 class StreamCopy:
     """What a block that sums its branches into the stream itself hands on instead of a pending
     sum: nothing is pending, and ``h`` is the residual stream as it stands, in the compute dtype
@@ -328,6 +349,12 @@ class Norm(Part):
     def forward(self, ctx: StepContext, x: torch.Tensor, delta: Optional[torch.Tensor]) -> torch.Tensor:
         raise NotImplementedError
 
+    offers_float8 = False        # True: forward_float8() is there
+
+    def forward_float8(self, ctx: StepContext, x: torch.Tensor, delta) -> Float8Rows:
+        """forward() with its result in 8 bits."""
+        raise NotImplementedError
+
     def add_normed(self, ctx: StepContext, x: torch.Tensor, a, b=None, want_copy: bool = False):
         """x += norm(a + b): the norm of a branch's *output* (a tensor, or float32 parts [P,T,H];
         ``b`` a second such source), summed into the float32 stream.  With ``want_copy`` returns
@@ -353,6 +380,8 @@ class Position(Part):
 
 
 class Mixer(Part):
+    offers_float8 = False        # True: the constructor takes weights="float8", and then the part has takes_float8
+    takes_float8 = False         # True: forward() wants h as Float8Rows
     takes_prenormed = False      # True: forward() accepts a Prenormed as h
     feeds_residual = False       # True: forward() accepts sink=ResidualSink and may return a Prenormed
     takes_riders = False         # True: set_riders() may be called once, after bind()
@@ -370,6 +399,8 @@ class Mixer(Part):
 
 
 class FeedForward(Part):
+    offers_float8 = False        # as for a mixer
+    takes_float8 = False
     takes_prenormed = False
     feeds_residual = False
 

@@ -20,6 +20,7 @@ class PreNormBlock(Block):
 
     norm_slots = ("norm_in", "norm_post")
     chains_norm = True
+    offers_float8 = True
 
     def __init__(self, mixer: Mixer, feed_forward: FeedForward, norm_in: Norm, norm_post: Norm):
         self.mixer, self.feed_forward, self.norm_in, self.norm_post = mixer, feed_forward, norm_in, norm_post
@@ -33,13 +34,17 @@ class PreNormBlock(Block):
     def first_norm(self):
         return self.norm_in
 
+    @staticmethod
+    def _normed(norm: Norm, part, ctx: StepContext, x: torch.Tensor, delta):
+        return norm.forward_float8(ctx, x, delta) if part.takes_float8 else norm.forward(ctx, x, delta)
+
     def forward(self, ctx: StepContext, x: torch.Tensor, delta, run: RunBinding, next_norm: Optional[Norm] = None):
-        h = self.norm_in.forward(ctx, x, delta)
+        h = self._normed(self.norm_in, self.mixer, ctx, x, delta)
         if isinstance(h, Prenormed) and not self.mixer.takes_prenormed:
             h = h.materialise(ctx)
         sink = self.norm_post.sink(ctx, x) if self.mixer.feeds_residual else None
         a = self.mixer.forward(ctx, h, run, sink=sink) if sink is not None else self.mixer.forward(ctx, h, run)
-        h2 = self.norm_post.forward(ctx, x, a)
+        h2 = self._normed(self.norm_post, self.feed_forward, ctx, x, a)
         if isinstance(h2, Prenormed) and not self.feed_forward.takes_prenormed:
             h2 = h2.materialise(ctx)
         sink = next_norm.sink(ctx, x) if (next_norm is not None and self.feed_forward.feeds_residual) else None
@@ -61,7 +66,7 @@ class PreNormMixerBlock(PreNormBlock):
         return {"norm_in": self.norm_in, "mixer": self.mixer}
 
     def forward(self, ctx: StepContext, x: torch.Tensor, delta, run: RunBinding, next_norm: Optional[Norm] = None):
-        h = self.norm_in.forward(ctx, x, delta)
+        h = self._normed(self.norm_in, self.mixer, ctx, x, delta)
         if isinstance(h, Prenormed) and not self.mixer.takes_prenormed:
             h = h.materialise(ctx)
         sink = next_norm.sink(ctx, x) if (next_norm is not None and self.mixer.feeds_residual) else None

@@ -8,12 +8,13 @@ the choice for debugging (``simple``, ``gemv``, ``tc``): it never selects a libr
 from __future__ import annotations
 
 import os
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
 
 from .. import kernels as K
-from .base import Prenormed, ResidualSink, StepContext
+from .base import Float8Rows, Prenormed, ResidualSink, StepContext
 
 _FORCE = os.environ.get("AIEN_B200_GEMM", "").strip().lower()
 
@@ -111,3 +112,38 @@ def linear_into_residual(ctx: StepContext, a: torch.Tensor, w: torch.Tensor, sin
     ssq = ctx.workspace.take((K.gemv_stream_grid(N), 16), torch.float32)
     parts = K.gemv_residual(a, w, sink.x, sink.weight, xw, ssq)
     return Prenormed(xw, ssq, parts, sink.eps, sink.norm)
+
+
+# ------------------------------------------------------------------ in 8 bits
+@dataclass
+class Float8Matrix:
+    """A weight [N, K] in 8 bits: e4m3 codes, every row on a 16-byte border, and a float32 scale for each 128 x 128 of it."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @staticmethod
+    def of(w: torch.Tensor) -> "Float8Matrix":
+        N, width = w.shape
+        codes = torch.empty((N, (width + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=w.device)[:, :width]
+        scales = torch.empty((K.float8_blocks(N), K.float8_blocks(width)), dtype=torch.float32, device=w.device)
+        K.quantize_blocks_float8(w, codes, scales)
+        return Float8Matrix(codes, scales)
+
+    def first_rows(self, n: int) -> "Float8Matrix":
+        return Float8Matrix(self.codes[:n], self.scales[:K.float8_blocks(n)])
+
+
+def float8_rows(ctx: StepContext, x: torch.Tensor) -> Float8Rows:
+    """x [T, K] in 8 bits, taken from the step workspace."""
+    rows = Float8Rows.take(ctx, x.shape[0], x.shape[1])
+    K.quantize_rows_float8(x, rows.codes, rows.scales)
+    return rows
+
+
+def linear_float8(ctx: StepContext, rows: Float8Rows, w: Float8Matrix, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """rows . w^T -> [T, N] taken from the step workspace.  Weights are never written during a step: the first of them are requested before the
+    kernel ahead is done."""
+    out = ctx.workspace.take((rows.codes.shape[0], w.codes.shape[0]), out_dtype)
+    K.matmul_float8(rows.codes, rows.scales, w.codes, w.scales, out, w_ready=True)
+    return out

@@ -7,21 +7,30 @@ from .. import kernels as K
 from ..registry import register_feed_forward
 from typing import Optional
 
-from .base import FeedForward, Prenormed, ResidualSink, StepContext
-from .linear import linear, linear_into_residual, linear_prenormed, _FORCE
+from .base import FeedForward, Float8Rows, Prenormed, ResidualSink, StepContext
+from .linear import Float8Matrix, linear, linear_float8, linear_into_residual, linear_prenormed, _FORCE
 
 
 @register_feed_forward("swiglu")
 class SwiGLU(FeedForward):
     """y = (act(h Wg^T) * (h Wu^T)) Wd^T with ``act`` "silu" (or "gelu_tanh", the tanh form of the gelu), no bias (crates/aien-inference-abi/src/
     transformer_backend.rs:1322-1362, silu in src/backend.rs:572-579).  gate and up are one
-    product over the stacked rows gate | up (src/resident.rs:284-288)."""
+    product over the stacked rows gate | up (src/resident.rs:284-288).
 
-    def __init__(self, hidden_size: int, intermediate_size: int, act: str = "silu"):
+    ``weights`` "float8": h comes in 8 bits, both matrices are kept and multiplied in 8 bits, and so is what lies between them (act(gate) * up is
+    float32 of the first product's bfloat16 result)."""
+
+    offers_float8 = True
+
+    def __init__(self, hidden_size: int, intermediate_size: int, act: str = "silu", weights: str = "stored"):
         self.hidden_size, self.intermediate_size = int(hidden_size), int(intermediate_size)
         if act not in K.GATED_ACTS:
             raise ValueError(f"activation {act!r}: known are {sorted(K.GATED_ACTS)}")
+        if weights not in ("stored", "float8"):
+            raise ValueError(f"weights {weights!r}: known are 'stored' and 'float8'")
         self.act, self.epilogue = act, K.GATED_ACTS[act]
+        if weights == "float8":
+            self.takes_float8, self.takes_prenormed, self.feeds_residual = True, False, False
         self.w_gate_up = self.w_down = None
 
     def param_shapes(self):
@@ -35,15 +44,20 @@ class SwiGLU(FeedForward):
         if g.dtype != u.dtype:
             g, u = g.float(), u.float()
         I, H = self.intermediate_size, self.hidden_size
-        self.group = self.GROUP if (g.dtype == torch.bfloat16 and I % self.GROUP == 0) else 0
+        self.group = self.GROUP if ((g.dtype == torch.bfloat16 or self.takes_float8) and I % self.GROUP == 0) else 0
         if self.group:
             n = I // self.group
             self.w_gate_up = torch.stack([g.view(n, self.group, H), u.view(n, self.group, H)], dim=1).reshape(2 * I, H).contiguous()
         else:
             self.w_gate_up = torch.cat([g, u], dim=0).contiguous()
         self.w_down = tensors["down_proj"].contiguous()
+        if self.takes_float8:
+            self.w_gate_up, self.w_down = Float8Matrix.of(self.w_gate_up), Float8Matrix.of(self.w_down)
 
     def workspace_bytes(self, lim):
+        if self.takes_float8:
+            return lim.max_tokens * (2 * self.intermediate_size + self.hidden_size) * lim.itemsize + 4096 \
+                + Float8Rows.workspace_bytes(lim, self.hidden_size) + Float8Rows.workspace_bytes(lim, self.intermediate_size)
         return lim.max_tokens * (3 * self.intermediate_size + self.hidden_size) * lim.itemsize + 4096 \
             + 8 * K.GEMV_MAX_ROWS * self.hidden_size * 4 + K.PARTIALS_MAX_BYTES + K.FUSED_NORM_SCRATCH_BYTES(self.hidden_size)
 
@@ -63,6 +77,11 @@ class SwiGLU(FeedForward):
         return act
 
     def forward(self, ctx: StepContext, h, sink: Optional[ResidualSink] = None):
+        if self.takes_float8:
+            gu = linear_float8(ctx, h, self.w_gate_up)
+            rows = Float8Rows.take(ctx, gu.shape[0], self.intermediate_size)
+            K.swiglu_float8(gu, rows.codes, rows.scales, self.group, self.act)
+            return linear_float8(ctx, rows, self.w_down)
         if isinstance(h, Prenormed):
             act = linear_prenormed(ctx, h, self.w_gate_up, epilogue=1) if self.group == 8 and self.act == "silu" else None
             if act is not None:

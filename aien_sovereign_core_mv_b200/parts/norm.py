@@ -7,7 +7,7 @@ import torch
 
 from .. import kernels as K
 from ..registry import register_norm
-from .base import Norm, NormedStream, Prenormed, ResidualSink, ScaledSum, StepContext, StreamCopy, SumTerms, add_to_residual
+from .base import Float8Rows, Norm, NormedStream, Prenormed, ResidualSink, ScaledSum, StepContext, StreamCopy, SumTerms, add_to_residual
 
 # AIEN_B200_FUSED_NORM=0 keeps every norm in its own kernel
 _FUSE = __import__("os").environ.get("AIEN_B200_FUSED_NORM", "1").strip() not in ("0", "off", "no")
@@ -78,6 +78,25 @@ class RMSNorm(Norm):
             return None
         return ResidualSink(x, self, self.weight, self.eps)
 
+    def _pending(self, ctx: StepContext, x: torch.Tensor, delta):
+        """What the norm's kernel still has to add to x."""
+        if isinstance(delta, StreamCopy):
+            return None                           # nothing pending
+        if isinstance(delta, (ScaledSum, SumTerms)):
+            add_to_residual(ctx, x, delta)        # left by a block that scales its branches or has several
+            return None
+        return delta
+
+    offers_float8 = True
+
+    def forward_float8(self, ctx: StepContext, x: torch.Tensor, delta) -> Float8Rows:
+        if isinstance(delta, (Prenormed, NormedStream)):
+            delta = None                          # x is up to date; what was made of it is in 16 bits
+        delta = self._pending(ctx, x, delta)
+        rows = Float8Rows.take(ctx, x.shape[0], x.shape[1])
+        K.add_rmsnorm_float8(x, delta, self.weight, self.eps, rows.codes, rows.scales)
+        return rows
+
     def forward(self, ctx: StepContext, x: torch.Tensor, delta):
         if isinstance(delta, Prenormed):
             if delta.norm is self:
@@ -87,11 +106,7 @@ class RMSNorm(Norm):
             if delta.norm is self:
                 return delta.h                    # made by the kernel that wrote the last sum
             delta = None
-        if isinstance(delta, StreamCopy):
-            delta = None                          # nothing pending
-        if isinstance(delta, (ScaledSum, SumTerms)):
-            add_to_residual(ctx, x, delta)        # left by a block that scales its branches or has several
-            delta = None
+        delta = self._pending(ctx, x, delta)
         out = ctx.workspace.take(tuple(x.shape), ctx.dtype)
         K.add_rmsnorm(x, delta, self.weight, self.eps, out)
         return out
