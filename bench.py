@@ -122,7 +122,7 @@ class ClockSampler:
                 "reasons": sorted(reasons), "samples": len(sm)}
 
 
-def model_numbers(cfg, layers_run):
+def model_numbers(cfg, layers_run, weights="stored"):
     H, I, V = cfg["hidden_size"], cfg["intermediate_size"], cfg["vocab_size"]
     Q = cfg["num_attention_heads"] * cfg["head_dim"]
     KV = cfg["num_key_value_heads"] * cfg["head_dim"]
@@ -130,7 +130,9 @@ def model_numbers(cfg, layers_run):
     linear_params = per_layer * layers_run + V * H                       # matrices a decode step reads
     norm_params = layers_run * (2 * H + (2 * cfg["head_dim"] if cfg["architectures"][0] == "Qwen3ForCausalLM" else 0)) + H
     kv_bytes_per_token = 2 * KV * 2 * layers_run
-    return dict(per_layer=per_layer, linear_params=linear_params, weight_bytes=2 * (linear_params + norm_params),
+    # 8-bit layers: a byte a number and a float32 scale for each block of 128 x 128; the head stays in 16 bits
+    layer_bytes = per_layer * layers_run * (1 + 4 / 128 ** 2) if weights == "float8" else 2 * per_layer * layers_run
+    return dict(per_layer=per_layer, linear_params=linear_params, weight_bytes=int(layer_bytes + 2 * (V * H + norm_params)),
                 kv_bytes_per_token=kv_bytes_per_token, Q=Q, KV=KV)
 
 
@@ -865,6 +867,8 @@ def main() -> int:
     ap.add_argument("--align-step-tokens", type=int, default=0,
                     help="serving workload: the scheduler cuts portions so that a step's tokens fill whole tiles of this many rows")
     ap.add_argument("--shape", default="", help="dulisun, ripesun, botalorn, mumazen, kuvidra and folavik workloads: only this shape (default: all)")
+    ap.add_argument("--weights", default="stored", choices=["stored", "float8"],
+                    help="decode and llama3_8b workloads: float8 keeps the layers' matrices in 8 bits (another computation than the default line's)")
     ap.add_argument("--skip-points", action="store_true")
     ap.add_argument("--skip-prefill", action="store_true")
     ap.add_argument("--skip-e2e", action="store_true")
@@ -929,14 +933,14 @@ def main() -> int:
     layers_cfg = cfg["num_hidden_layers"]
     layers_run = args.layers or layers_cfg
     cfg["num_hidden_layers"] = layers_run
-    nums = model_numbers(cfg, layers_run)
+    nums = model_numbers(cfg, layers_run, args.weights)
     hbm_gbs, bf16_tflops, peak_src = peaks()
     CONTEXT, SEED = wl["context"], wl["seed"]
     # the timed steps end at `context` tokens when the workload gives no prompt length
     PROMPT_LEN = wl["prompt_len"] or CONTEXT - (warmup + steps)
     max_batch = max([batch_main, *wl["points"]])
     pool_tokens = max_batch * (PROMPT_LEN + warmup + steps + 64) + ptok
-    ec = EngineConfig(dtype="bfloat16", page_size=PAGE, max_cache_tokens=pool_tokens, max_requests=max_batch,
+    ec = EngineConfig(dtype="bfloat16", weights=args.weights, page_size=PAGE, max_cache_tokens=pool_tokens, max_requests=max_batch,
                       max_batch_tokens=max(PREFILL_TOKENS, ptok), max_context=CONTEXT + (0 if wl["prompt_len"] else 64), max_batch_size=max_batch,
                       max_prefill_tokens=max(PREFILL_TOKENS, ptok), prefill_chunk_size=max(PREFILL_TOKENS, ptok))
     t_load = time.time()
@@ -1099,14 +1103,14 @@ def main() -> int:
     out = {
         "metric": "decode_tokens_per_s", "value": round(value, 1), "unit": "tokens/s", "n_gpus": 1, "steps": steps,
         "warmup": warmup, "ms_per_step": round(ms_per_step, 4), "higher_is_better": True, "scaling": "weak",
-        "vs_baseline": None, "dtype": "bf16", "data": "synthetic", "impl": "ours",
+        "vs_baseline": None, "dtype": "bf16" if args.weights == "stored" else "e4m3 layers, bf16", "data": "synthetic", "impl": "ours",
         "config": {
-            "model": wl["label"], "layers": layers_cfg, "layers_run": layers_run,
+            "model": wl["label"], "weights": args.weights, "layers": layers_cfg, "layers_run": layers_run,
             "hidden": cfg["hidden_size"], "heads": cfg["num_attention_heads"], "kv_heads": cfg["num_key_value_heads"],
             "head_dim": cfg["head_dim"], "intermediate": cfg["intermediate_size"], "vocab": V,
             "global_batch": batch_main, "seq_len": PROMPT_LEN, "context": CONTEXT, "page_size": PAGE,
             "parallelism": "single GPU", "prefill_tokens": ptok, "seed": SEED,
-            "l2": "inputs larger than L2: 15 GB of weights per step", "fill": args.fill,
+            "l2": f"inputs larger than L2: {round(nums['weight_bytes'] / 1e9)} GB of weights per step", "fill": args.fill,
         },
         "clocks": clocks, "e2e": e2e, "gpu_launches": int(launches), "wait_errors": int(wait_errors),
         "prefill": prefill,
