@@ -20,8 +20,9 @@ constexpr float F8_TOP = 448.0f, F8_LEAST = 1.17549435e-38f;      // the largest
 
 __device__ __forceinline__ uint32_t f8_bits(float v) { return __float_as_uint(fabsf(v)); }
 __device__ __forceinline__ float f8_scale(uint32_t top) {
-    return top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__fdiv_rn(__uint_as_float(top), F8_TOP), F8_LEAST);
+    return top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(top) * (1.0f / F8_TOP), F8_LEAST);
 }
+__device__ __forceinline__ float f8_inverse(float scale) { return __frcp_rn(scale); }
 __device__ __forceinline__ uint32_t f8_pair(float a, float b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
@@ -36,61 +37,72 @@ __device__ __forceinline__ uint32_t f8_half_max(uint32_t v) {
     return v;
 }
 
-// Eight numbers as one or two 16-byte loads.  __ldcg: what an earlier kernel of a chain wrote (see common.cuh).
-__device__ __forceinline__ void f8_load8(const float* p, float v[8]) {
-    const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void f8_load8(const __nv_bfloat16* p, float v[8]) {
-    const uint4 r = __ldcg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+// Eight numbers as they lie in memory, one or two 16-byte loads.  __ldcg: what an earlier kernel of a chain wrote (see common.cuh).
+template <typename T> struct F8Raw;
+template <> struct F8Raw<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = __ldcg(reinterpret_cast<const float4*>(p));
+        b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
     }
+    __device__ __forceinline__ void get(float v[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+template <> struct F8Raw<__nv_bfloat16> {
+    uint4 r;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { r = __ldcg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void get(float v[8]) const {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+template <typename T>
+__device__ __forceinline__ void f8_load8(const T* p, float v[8]) {
+    F8Raw<T> r;
+    r.load(p);
+    r.get(v);
 }
 
 // ---------------------------------------------------------------- rows, and gated activations of rows
-// Where the eight numbers of a lane come from.  VEC: eight neighbours, loaded whole (every row starts on a 16-byte border and holds whole
-// eights); otherwise numbers lane, lane + 16, ... of the block, one by one.
-template <typename T, bool VEC> struct F8Plain {
+// Where the eight numbers of a lane come from.  Eight neighbours, loaded whole, where every row starts on a 16-byte border and holds whole eights (load and
+// get); otherwise numbers lane, lane + 16, ... of the block, one by one (each).
+template <typename T> struct F8Plain {
     const T* x;
     long ld;
-    __device__ __forceinline__ void get(long t, int k0, int lane, int K, float v[8]) const {
-        const T* p = x + t * ld;
-        if (VEC) {
-            f8_load8(p + k0 + lane * 8, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k0 + j * 16 + lane < K ? ld_act(p + k0 + j * 16 + lane) : 0.f;
-        }
-    }
+    struct Raw { F8Raw<T> x; };
+    __device__ __forceinline__ void load(long t, int i, int K, Raw& r) const { r.x.load(x + t * ld + i); }
+    __device__ __forceinline__ void get(const Raw& r, float v[8]) const { r.x.get(v); }
+    __device__ __forceinline__ float each(long t, int i, int K) const { return ld_act(x + t * ld + i); }
 };
 __device__ __forceinline__ float f8_gate(float g, float u, int gelu) {
     const float f = gelu ? 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) : __fdividef(g, 1.0f + __expf(-g));
     return f * u;
 }
-template <typename T, bool VEC> struct F8Gated {
+template <typename T> struct F8Gated {
     const T* gu;
     int group, gelu;
-    __device__ __forceinline__ void get(long t, int k0, int lane, int K, float v[8]) const {
+    struct Raw { F8Raw<T> g, u; };
+    __device__ __forceinline__ void load(long t, int i, int K, Raw& r) const {
         const T* p = gu + t * 2 * (long)K;
-        if (VEC) {
-            const int i = k0 + lane * 8;
-            float g[8], u[8];
-            f8_load8(p + (group == 0 ? i : 2 * i), g);
-            f8_load8(p + (group == 0 ? K + i : 2 * i + 8), u);
+        r.g.load(p + (group == 0 ? i : 2 * i));
+        r.u.load(p + (group == 0 ? K + i : 2 * i + 8));
+    }
+    __device__ __forceinline__ void get(const Raw& r, float v[8]) const {
+        float u[8];
+        r.g.get(v);
+        r.u.get(u);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = f8_gate(g[j], u[j], gelu);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int i = k0 + j * 16 + lane;
-                const long gi = group == 0 ? i : (long)(i / group) * 2 * group + i % group;
-                v[j] = i < K ? f8_gate(ld_act(p + gi), ld_act(p + gi + (group == 0 ? K : group)), gelu) : 0.f;
-            }
-        }
+        for (int j = 0; j < 8; ++j) v[j] = f8_gate(v[j], u[j], gelu);
+    }
+    __device__ __forceinline__ float each(long t, int i, int K) const {
+        const T* p = gu + t * 2 * (long)K;
+        const long gi = group == 0 ? i : (long)(i / group) * 2 * group + i % group;
+        return f8_gate(ld_act(p + gi), ld_act(p + gi + (group == 0 ? K : group)), gelu);
     }
 };
 
@@ -107,54 +119,84 @@ __device__ __forceinline__ void f8_store(uint8_t* codes, int k0, int lane, int K
     }
 }
 
-// Half a warp takes a block of a row.  A CTA's 16 halves are `rows` rows times 16 / rows neighbouring blocks (rows a power of two), so
-// that the scales of a block, which lie side by side over the rows, leave together.
-template <typename SRC, bool VEC>
+// Half a warp takes a block of a row, U blocks of it one after the other whose loads are all on their way first.  A CTA's 16 halves are `rows` rows times
+// 16 / rows neighbouring blocks (rows a power of two), so that the scales of a block, which lie side by side over the rows, leave together.
+// (As many CTAs as the GPU holds, walking over the blocks with the next one's numbers on their way, took longer: 2,048 x 12,288 gated in 37 us.)
+template <typename SRC, bool VEC, int U>
 __global__ void __launch_bounds__(256)
 rows_float8_kernel(SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, int rows) {
     griddep_launch();
     griddep_wait();
-    const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    const int half = threadIdx.x >> 4, lane = threadIdx.x & 15, wide = 16 / rows;
     const long t = (long)blockIdx.x * rows + half % rows;
-    const int b = blockIdx.y * (16 / rows) + half / rows, k0 = b * F8_BLOCK;
-    const bool live = t < T && k0 < K;
-    float v[8];
+    const int b0 = blockIdx.y * wide * U + half / rows;
+    typename SRC::Raw raw[U];
+    if (VEC) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    const bool mine = live && (!VEC || k0 + lane * 8 < K);
-    if (mine) src.get(t, k0, lane, K, v);
-    uint32_t top = 0;
+        for (int u = 0; u < U; ++u) {
+            const int i = (b0 + u * wide) * F8_BLOCK + lane * 8;
+            if (t < T && i < K) src.load(t, i, K, raw[u]);
+        }
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, f8_bits(v[j]));
-    top = f8_half_max(top);
-    const float s = f8_scale(top), inv = __fdiv_rn(1.0f, s);
-    if (mine) f8_store<VEC>(codes + t * ldq, k0, lane, K, v, inv);
-    if (live && lane == 0) scales[(long)b * lds + t] = s;
+    for (int u = 0; u < U; ++u) {
+        const int b = b0 + u * wide, k0 = b * F8_BLOCK;
+        const bool mine = t < T && (VEC ? k0 + lane * 8 < K : k0 < K);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        if (mine) {
+            if (VEC) {
+                src.get(raw[u], v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (k0 + j * 16 + lane < K) v[j] = src.each(t, k0 + j * 16 + lane, K);
+            }
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, f8_bits(v[j]));
+        top = f8_half_max(top);
+        const float s = f8_scale(top), inv = f8_inverse(s);
+        if (mine) f8_store<VEC>(codes + t * ldq, k0, lane, K, v, inv);
+        if (t < T && k0 < K && lane == 0) scales[(long)b * lds + t] = s;
+    }
 }
 
-template <typename SRC, bool VEC>
-static int launch_rows_float8(SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, cudaStream_t stream) {
+template <typename SRC, bool VEC, int U>
+static int launch_rows_float8_by(SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, cudaStream_t stream) {
     const int blocks = (K + F8_BLOCK - 1) / F8_BLOCK;
     int rows = 1;
     while (rows < 8 && rows < T) rows *= 2;
-    const long gx = ((long)T + rows - 1) / rows, gy = ((long)blocks + 16 / rows - 1) / (16 / rows);
+    const int each = 16 / rows * U;
+    const long gx = ((long)T + rows - 1) / rows, gy = ((long)blocks + each - 1) / each;
     if (gy > 65535) return AIEN_E_SHAPE;
-    launch_chain(rows_float8_kernel<SRC, VEC>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, stream, src, codes, ldq, scales, lds, T, K, rows);
+    launch_chain(rows_float8_kernel<SRC, VEC, U>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, stream, src, codes, ldq, scales, lds, T, K, rows);
     return launch_status();
+}
+// Two blocks a half from two loads of the GPU on (148 SMs of 128 halves): gated, 2,048 x 12,288 in 31.4 us by one and 27.7 by two (by four 28.4), 512 x 12,288 in
+// 9.3 and 8.8, but 64 x 12,288 in 2.5 and 3.2; rows of 2,048 x 4,096 in 8.1 and 7.0, of 512 x 4,096 in 3.0 and 3.5.
+template <typename SRC>
+static int launch_rows_float8(bool vec, SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, cudaStream_t stream) {
+    if (!vec) return launch_rows_float8_by<SRC, false, 1>(src, codes, ldq, scales, lds, T, K, stream);
+    if ((long)T * ((K + F8_BLOCK - 1) / F8_BLOCK) >= 2L * 148 * 128) return launch_rows_float8_by<SRC, true, 2>(src, codes, ldq, scales, lds, T, K, stream);
+    return launch_rows_float8_by<SRC, true, 1>(src, codes, ldq, scales, lds, T, K, stream);
 }
 
 // ---------------------------------------------------------------- the residual's sum and its norm
 // x += sum of the parts; h = x / sqrt(mean x^2 + eps) * w; codes and scales of h.  One CTA a row, the row in registers (NV times eight
 // numbers a thread) between the sum of squares and the codes; a block of 128 lies in half a warp.
-template <typename TD, int NV, int BS>
+template <typename TD, typename TW, int NV, int BS>
 __global__ void __launch_bounds__(BS)
-add_rmsnorm_float8_vec_kernel(float* x, const TD* delta, int nparts, size_t part_stride, const void* w, int wdt, float eps,
+add_rmsnorm_float8_vec_kernel(float* x, const TD* delta, int nparts, size_t part_stride, const TW* w, float eps,
                               uint8_t* codes, long ldq, float* scales, long lds, int H) {
     __shared__ float red[32];
     griddep_launch();
     griddep_wait();
     const size_t base = (size_t)blockIdx.x * H;
     float v[NV][8];
+    F8Raw<TW> wv[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int i = (j * BS + threadIdx.x) * 8;
@@ -185,7 +227,9 @@ add_rmsnorm_float8_vec_kernel(float* x, const TD* delta, int nparts, size_t part
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss += v[j][e] * v[j][e];
         const int i = (j * BS + threadIdx.x) * 8;
-        if (delta != nullptr && i < H) {
+        if (i >= H) continue;
+        wv[j].load(w + i);                                                  // on its way while the sum is made
+        if (delta != nullptr) {
             float4* o = reinterpret_cast<float4*>(x + base + i);
             o[0] = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
             o[1] = make_float4(v[j][4], v[j][5], v[j][6], v[j][7]);
@@ -197,17 +241,16 @@ add_rmsnorm_float8_vec_kernel(float* x, const TD* delta, int nparts, size_t part
         const int i = (j * BS + threadIdx.x) * 8;
         uint32_t top = 0;
         if (i < H) {
-            float wv[8];
-            if (wdt == AIEN_DT_F32) f8_load8(reinterpret_cast<const float*>(w) + i, wv);
-            else f8_load8(reinterpret_cast<const __nv_bfloat16*>(w) + i, wv);
+            float g[8];
+            wv[j].get(g);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[j][e] = v[j][e] * rstd * wv[e];
+                v[j][e] = v[j][e] * rstd * g[e];
                 top = max(top, f8_bits(v[j][e]));
             }
         }
         top = f8_half_max(top);
-        const float s = f8_scale(top), inv = __fdiv_rn(1.0f, s);
+        const float s = f8_scale(top), inv = f8_inverse(s);
         if (i < H) {
             *reinterpret_cast<uint2*>(codes + (size_t)blockIdx.x * ldq + i) = f8_pack(v[j], inv);
             if ((threadIdx.x & 15) == 0) scales[(long)(i / F8_BLOCK) * lds + blockIdx.x] = s;
@@ -247,7 +290,7 @@ add_rmsnorm_float8_kernel(float* x, const TD* delta, int nparts, size_t part_str
             top = max(top, f8_bits(v[j]));
         }
         top = f8_half_max(top);
-        const float s = f8_scale(top), inv = __fdiv_rn(1.0f, s);
+        const float s = f8_scale(top), inv = f8_inverse(s);
         f8_store<false>(codes + (size_t)blockIdx.x * ldq, k0, lane, H, v, inv);
         if (lane == 0 && b < blocks) scales[(long)b * lds + blockIdx.x] = s;
     }
@@ -258,49 +301,70 @@ static int launch_add_rmsnorm_float8(float* x, const TD* delta, int nparts, size
                                      uint8_t* codes, long ldq, float* scales, long lds, int T, int H, cudaStream_t stream) {
     const bool vec = H % 8 == 0 && part_stride % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)codes & 7) == 0 &&
                      (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)w) & 15) == 0;
-#define F8_NORM(NV, BS)                                                                                                              \
-    launch_chain(add_rmsnorm_float8_vec_kernel<TD, NV, BS>, dim3(T), dim3(BS), 0, stream, x, delta, nparts, part_stride, w, w_dt, eps, \
+#define F8_NORM_W(TW, NV, BS)                                                                                                               \
+    launch_chain(add_rmsnorm_float8_vec_kernel<TD, TW, NV, BS>, dim3(T), dim3(BS), 0, stream, x, delta, nparts, part_stride, (const TW*)w, eps, \
                  codes, ldq, scales, lds, H)
+#define F8_NORM(NV, BS)                              \
+    do {                                             \
+        if (w_dt == AIEN_DT_F32) F8_NORM_W(float, NV, BS); \
+        else F8_NORM_W(__nv_bfloat16, NV, BS);       \
+    } while (0)
+    // Many rows of up to 4,096: sixteen numbers a thread, whose loads are more (512 rows in 6.5 us for 7.1, 8,192 in 59.3 for 62.0); few: eight (64 in 2.7 for 2.75).
     if (vec && H <= 8 * 256) F8_NORM(1, 256);
+    else if (vec && H <= 16 * 256 && T >= 512) F8_NORM(2, 256);
     else if (vec && H <= 8 * 512) F8_NORM(1, 512);
     else if (vec && H <= 16 * 512) F8_NORM(2, 512);
     else if (vec && H <= 32 * 512) F8_NORM(4, 512);
     else
         launch_chain(add_rmsnorm_float8_kernel<TD>, dim3(T), dim3(512), 0, stream, x, delta, nparts, part_stride, w, w_dt, eps, codes, ldq, scales, lds, H);
+#undef F8_NORM_W
 #undef F8_NORM
     return launch_status();
 }
 
 // ---------------------------------------------------------------- weights
-// A CTA takes a block of 128 x 128: 16 lanes a row of it, 16 rows at a time, the whole block in registers until its maximum is known.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+// A CTA takes a block of 128 x 128: 16 lanes a row of it, BS / 16 rows at a time, the whole block in registers until its maximum is known, as it lies in
+// memory where it is loaded in eights (256 threads), number by number otherwise (1,024 threads, sixteen numbers each).
+template <typename T, bool VEC, int BS>
+__global__ void __launch_bounds__(BS)
 blocks_float8_kernel(const T* w, long ldw, uint8_t* codes, long ldq, float* scales, long lds, int N, int K) {
-    __shared__ uint32_t tops[8];
-    const int n0 = blockIdx.y * F8_BLOCK, k0 = blockIdx.x * F8_BLOCK;
-    const int r = threadIdx.x >> 4, lane = threadIdx.x & 15;
-    float v[8][8];
+    constexpr int PASSES = 2048 / BS;
+    __shared__ uint32_t tops[32];
+    const int n0 = blockIdx.y * F8_BLOCK + (threadIdx.x >> 4), k0 = blockIdx.x * F8_BLOCK, lane = threadIdx.x & 15;
+    F8Raw<T> raw[VEC ? PASSES : 1];
+    float v[VEC ? 1 : PASSES][8];
+    auto mine = [&](int i) { return n0 + i * (BS / 16) < N && (!VEC || k0 + lane * 8 < K); };
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const T* p = w + (long)(n0 + i * (BS / 16)) * ldw + k0;
+        if (VEC) {
+            if (mine(i)) raw[i].load(p + lane * 8);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = mine(i) && k0 + j * 16 + lane < K ? ld_act(p + j * 16 + lane) : 0.f;
+        }
+    }
     uint32_t top = 0;
-    const F8Plain<T, VEC> src{w, ldw};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int n = n0 + i * 16 + r;
+    for (int i = 0; i < PASSES; ++i) {
+        float (&u)[8] = v[VEC ? 0 : i];
+        if (!mine(i)) continue;
+        if (VEC) raw[i].get(u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-        if (n < N && (!VEC || k0 + lane * 8 < K)) src.get(n, k0, lane, K, v[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, f8_bits(v[i][j]));
+        for (int j = 0; j < 8; ++j) top = max(top, f8_bits(u[j]));
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
-    const float s = f8_scale(top), inv = __fdiv_rn(1.0f, s);
+    for (int i = 0; i < BS / 32; ++i) top = max(top, tops[i]);
+    const float s = f8_scale(top), inv = f8_inverse(s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int n = n0 + i * 16 + r;
-        if (n < N && (!VEC || k0 + lane * 8 < K)) f8_store<VEC>(codes + (long)n * ldq, k0, lane, K, v[i], inv);
+    for (int i = 0; i < PASSES; ++i) {
+        float (&u)[8] = v[VEC ? 0 : i];
+        if (!mine(i)) continue;
+        if (VEC) raw[i].get(u);
+        f8_store<VEC>(codes + (long)(n0 + i * (BS / 16)) * ldq, k0, lane, K, u, inv);
     }
     if (threadIdx.x == 0) scales[(long)blockIdx.y * lds + blockIdx.x] = s;
 }
@@ -314,9 +378,8 @@ AIEN_API int aien_quantize_rows_float8(const void* x, int dt, long ldx, void* co
     if (T <= 0) return 0;
     if (K <= 0) return AIEN_E_SHAPE;
     const bool ends = K % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)x & 15) == 0;
-#define F8_ROWS(TX, WHOLE)                                                                                                                      \
-    return ends && ldx % WHOLE == 0 ? launch_rows_float8<F8Plain<TX, true>, true>({(const TX*)x, ldx}, (uint8_t*)codes, ldq, scales, lds, T, K, stream) \
-                                    : launch_rows_float8<F8Plain<TX, false>, false>({(const TX*)x, ldx}, (uint8_t*)codes, ldq, scales, lds, T, K, stream)
+#define F8_ROWS(TX, WHOLE) \
+    return launch_rows_float8(ends && ldx % WHOLE == 0, F8Plain<TX>{(const TX*)x, ldx}, (uint8_t*)codes, ldq, scales, lds, T, K, stream)
     if (dt == AIEN_DT_F32) F8_ROWS(float, 4);
     if (dt == AIEN_DT_BF16) F8_ROWS(__nv_bfloat16, 8);
 #undef F8_ROWS
@@ -328,9 +391,7 @@ AIEN_API int aien_swiglu_float8(const void* gu, int dt, int group, int gelu, voi
     if (T <= 0) return 0;
     if (K <= 0 || group < 0 || (group > 0 && K % group != 0)) return AIEN_E_SHAPE;
     const bool vec = K % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)gu & 15) == 0 && (group == 0 || group == 8);
-#define F8_GATED(TX)                                                                                                                             \
-    return vec ? launch_rows_float8<F8Gated<TX, true>, true>({(const TX*)gu, group, gelu}, (uint8_t*)codes, ldq, scales, lds, T, K, stream)            \
-               : launch_rows_float8<F8Gated<TX, false>, false>({(const TX*)gu, group, gelu}, (uint8_t*)codes, ldq, scales, lds, T, K, stream)
+#define F8_GATED(TX) return launch_rows_float8(vec, F8Gated<TX>{(const TX*)gu, group, gelu}, (uint8_t*)codes, ldq, scales, lds, T, K, stream)
     if (dt == AIEN_DT_F32) F8_GATED(float);
     if (dt == AIEN_DT_BF16) F8_GATED(__nv_bfloat16);
 #undef F8_GATED
@@ -356,8 +417,8 @@ AIEN_API int aien_quantize_blocks_float8(const void* w, int dt, long ldw, void* 
     const bool ends = K % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)w & 15) == 0;
 #define F8_BLOCKS(TX, WHOLE)                                                                                                        \
     do {                                                                                                                            \
-        if (ends && ldw % WHOLE == 0) blocks_float8_kernel<TX, true><<<grid, 256, 0, stream>>>((const TX*)w, ldw, (uint8_t*)codes, ldq, scales, lds, N, K); \
-        else blocks_float8_kernel<TX, false><<<grid, 256, 0, stream>>>((const TX*)w, ldw, (uint8_t*)codes, ldq, scales, lds, N, K); \
+        if (ends && ldw % WHOLE == 0) blocks_float8_kernel<TX, true, 256><<<grid, 256, 0, stream>>>((const TX*)w, ldw, (uint8_t*)codes, ldq, scales, lds, N, K); \
+        else blocks_float8_kernel<TX, false, 1024><<<grid, 1024, 0, stream>>>((const TX*)w, ldw, (uint8_t*)codes, ldq, scales, lds, N, K); \
         return launch_status();                                                                                                     \
     } while (0)
     if (dt == AIEN_DT_F32) F8_BLOCKS(float, 4);
