@@ -10,26 +10,10 @@
 //
 // All of these are bound by memory, or for a few rows by latency: every number is read once, kept in registers while its block's
 // (or row's) maximum is found, and written once.
-#include "common.cuh"
-#include <cuda_fp8.h>
+#include "float8.cuh"
 
 namespace aien {
 
-constexpr int F8_BLOCK = 128;
-constexpr float F8_TOP = 448.0f, F8_LEAST = 1.17549435e-38f;      // the largest e4m3 number; 2^-126
-
-__device__ __forceinline__ uint32_t f8_bits(float v) { return __float_as_uint(fabsf(v)); }
-__device__ __forceinline__ float f8_scale(uint32_t top) {
-    return top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(top) * (1.0f / F8_TOP), F8_LEAST);
-}
-__device__ __forceinline__ float f8_inverse(float scale) { return __frcp_rn(scale); }
-__device__ __forceinline__ uint32_t f8_pair(float a, float b) {
-    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ uint2 f8_pack(const float v[8], float inv) {
-    return make_uint2(f8_pair(v[0] * inv, v[1] * inv) | f8_pair(v[2] * inv, v[3] * inv) << 16,
-                      f8_pair(v[4] * inv, v[5] * inv) | f8_pair(v[6] * inv, v[7] * inv) << 16);
-}
 // maximum over the 16 lanes that share a block
 __device__ __forceinline__ uint32_t f8_half_max(uint32_t v) {
 #pragma unroll

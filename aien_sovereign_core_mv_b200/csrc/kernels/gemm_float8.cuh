@@ -13,6 +13,7 @@
 // Rows and columns beyond the matrices are zero-filled by TMA, stores are masked.  Rows of codes that do not all start on 16-byte borders
 // are brought by threads in TMA's place (f8_gather).
 #pragma once
+#include "float8.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -456,13 +457,58 @@ struct F8Rows {
     long ldw;
 };
 
+// Where a gated product's result goes: codes [M, N / 2] and scales [ceil(N / 256), M].
+struct F8Gated8 {
+    uint8_t* codes;
+    long ldq;
+    float* scales;
+    long lds;
+    int gelu;
+};
+// act(gate) * up of a row's 128 columns, which hold gate and up in runs of 8, in 8 bits.  A tile's 256 columns give the 128 numbers of one block: the two
+// threads of a row tell each other their largest (`tops`, two floats a row).  All of it is float32: the columns are never rounded to 16 bits.
+__device__ __forceinline__ void f8_store_gated(float (&acc)[128], const F8Gated8& g, uint32_t tops, int half, int row, int m, int n, int M, int N) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float z = acc[16 * v + j], u = acc[16 * v + 8 + j];
+            const float y = (g.gelu ? 0.5f * z * (1.0f + tanh_ex2(0.7978845608028654f * (z + 0.044715f * z * z * z))) : __fdividef(z, 1.0f + __expf(-z))) * u;
+            acc[8 * v + j] = y;
+            if (n + 16 * v < N) top = max(top, f8_bits(y));
+        }
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(tops + (half * 128 + row) * 4), "r"(top) : "memory");
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    uint32_t other;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(other) : "r"(tops + ((half ^ 1) * 128 + row) * 4) : "memory");
+    const float s = f8_scale(max(top, other)), inv = f8_inverse(s);
+    if (m >= M) return;
+    if (half == 0) g.scales[(long)(n / 256) * g.lds + m] = s;
+    uint8_t* to = g.codes + (long)m * g.ldq + n / 2;
+    const bool whole = ((uintptr_t)to & 7) == 0;
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+        if (n + 16 * v >= N) continue;
+        const uint2 c = f8_pack(&acc[8 * v], inv);
+        if (whole) {
+            *reinterpret_cast<uint2*>(to + 8 * v) = c;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to[8 * v + j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+        }
+    }
+}
+
 // Persistent.  Warp 0 fetches, warp 1 multiplies, warp 2 brings the scales, warps 4 to 11 add up: each a quarter of the tile's rows times half
 // of its columns, a row a thread; they take the registers that the first four give up.  GATHER: four more warps fetch in warp 0's place.
-template <bool PAIR, bool GATHER, typename TC>
+// GATED (in pairs): W's rows are gate and up in runs of 8, the result is act(gate) * up in 8 bits.
+template <bool PAIR, bool GATHER, bool GATED, typename TC>
 __global__ void __launch_bounds__(GATHER ? 512 : 384, 1)
 float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
-                    int store_by_tma, F8Scales sc, TC* __restrict__ out, long ldc, int M, int N, int K, int m_tiles, int tiles, F8Rows rows) {
+                    int store_by_tma, F8Scales sc, TC* __restrict__ out, long ldc, int M, int N, int K, int m_tiles, int tiles, F8Rows rows, F8Gated8 gated) {
     static_assert(!(PAIR && GATHER), "rows that start anywhere are multiplied in tiles of one CTA");
+    static_assert(PAIR || !GATED, "a block of a gated result is 256 columns");
     using C = F8Tiles<PAIR>;
     constexpr int P = C::P;
     extern __shared__ uint8_t smem_raw[];
@@ -595,6 +641,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         constexpr int W = 64 * P;                                             // a thread's columns
         const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
         const uint32_t buf = sStore + (warp - 4) * F8_STORE;
+        uint32_t turn = 0;
         const uint32_t columns = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * W);
         const uint32_t factors = sScale + row * (F8_BATCH * 4), factors_w = sScale + (128 + (PAIR ? half : 0)) * (F8_BATCH * 4);
         F8Ring<C::BUFS> t;
@@ -625,8 +672,13 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 });
                 f = make_float4(f.y, f.z, f.w, 0.f);
             }
-            f8_store_rows<W, TC>(acc, &map_out, store_by_tma != 0, buf, out, ldc, tile % m_tiles * C::BM + rank * 128 + quarter * 32,
-                                 tile / m_tiles * C::BN + half * W, M, N);
+            const int m = tile % m_tiles * C::BM + rank * 128, n = tile / m_tiles * C::BN + half * W;
+            if constexpr (GATED) {
+                // (two places for the largest numbers in turn: whoever writes one again has met everyone behind the reading of it)
+                f8_store_gated(acc, gated, sStore + (turn++ & 1) * 1024, half, row, m + row, n, M, N);
+            } else {
+                f8_store_rows<W, TC>(acc, &map_out, store_by_tma != 0, buf, out, ldc, m + quarter * 32, n, M, N);
+            }
         }
         if (lane == 0) tma_store_done();
     }
@@ -698,21 +750,21 @@ int launch_float8_few(const void* a, long lda, const void* w, long ldw, F8Scales
     return f8_launch(kernel, dim3(Z, (unsigned)m_tiles, (unsigned)n_tiles), 192, F8Few<NT>::SMEM, Z, stream, ma, mw, sc, (TC*)out, ldc, M, N, K, w_ready);
 }
 
-template <bool PAIR, bool GATHER, typename TC>
-int launch_float8_tiles(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, cudaStream_t stream) {
+template <bool PAIR, bool GATHER, bool GATED, typename TC>
+int launch_float8_tiles(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, F8Gated8 gated, cudaStream_t stream) {
     using C = F8Tiles<PAIR>;
     constexpr int P = C::P;
     CUtensorMap ma = {}, mw = {}, mo = {};
     if (!GATHER && (!f8_make_map(&ma, a, M, K, lda, 128) || !f8_make_map(&mw, w, N, K, ldw, 128))) return AIEN_E_STATE;
-    const bool by_tma = ((uintptr_t)out & 15) == 0 && (M == 1 || ldc * sizeof(TC) % 16 == 0);
+    const bool by_tma = !GATED && ((uintptr_t)out & 15) == 0 && (M == 1 || ldc * sizeof(TC) % 16 == 0);
     if (by_tma && !f8_make_map_out<TC>(&mo, out, M, N, ldc)) return AIEN_E_STATE;
-    constexpr auto kernel = float8_tiles_kernel<PAIR, GATHER, TC>;
+    constexpr auto kernel = float8_tiles_kernel<PAIR, GATHER, GATED, TC>;
     if (!f8_configure<kernel, C::SMEM>()) return AIEN_E_STATE;
     const long m_tiles = ((long)M + C::BM - 1) / C::BM, tiles = m_tiles * (((long)N + C::BN - 1) / C::BN);
     if (tiles > 2147483647L) return AIEN_E_SHAPE;
     const long at_once = f8_sms() / P;
     return f8_launch(kernel, dim3((unsigned)((tiles < at_once ? tiles : at_once) * P)), GATHER ? 512 : 384, C::SMEM, P, stream, ma, mw, mo, (int)by_tma, sc,
-                     (TC*)out, ldc, M, N, K, (int)m_tiles, (int)tiles, F8Rows{(const uint8_t*)a, lda, (const uint8_t*)w, ldw});
+                     (TC*)out, ldc, M, N, K, (int)m_tiles, (int)tiles, F8Rows{(const uint8_t*)a, lda, (const uint8_t*)w, ldw}, gated);
 }
 
 // The product's form, by the time that each would take (us; measured with K of 4,096 and 12,288 on rows of 8 to 4,096, with one to three waves):
@@ -744,18 +796,22 @@ inline F8Plan f8_plan(int M, int N, int K) {
     return t1 <= t2 ? F8Plan{1, 1} : F8Plan{2, 1};
 }
 
+// every row of codes starts on a 16-byte border
+inline bool f8_whole_rows(const void* a, long lda, const void* w, long ldw, int M, int N) {
+    return (((uintptr_t)a | (uintptr_t)w) & 15) == 0 && (M == 1 || lda % 16 == 0) && (N == 1 || ldw % 16 == 0);
+}
+
 template <typename TC>
 int launch_float8(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, int w_ready, cudaStream_t stream) {
-    const bool whole = (((uintptr_t)a | (uintptr_t)w) & 15) == 0 && (M == 1 || lda % 16 == 0) && (N == 1 || ldw % 16 == 0);
-    if (!whole) return launch_float8_tiles<false, true, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream);
+    if (!f8_whole_rows(a, lda, w, ldw, M, N)) return launch_float8_tiles<false, true, false, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, F8Gated8{}, stream);
     const F8Plan plan = f8_plan(M, N, K);
 #define F8_FEW(NT) return launch_float8_few<NT, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, plan.Z, w_ready, stream)
     if (plan.form == 16) F8_FEW(16);
     if (plan.form == 32) F8_FEW(32);
     if (plan.form == 64) F8_FEW(64);
 #undef F8_FEW
-    if (plan.form == 1) return launch_float8_tiles<false, false, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream);
-    return launch_float8_tiles<true, false, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, stream);
+    if (plan.form == 1) return launch_float8_tiles<false, false, false, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, F8Gated8{}, stream);
+    return launch_float8_tiles<true, false, false, TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, F8Gated8{}, stream);
 }
 
 }  // namespace aien
@@ -770,4 +826,21 @@ AIEN_API int aien_matmul_float8(const void* a, long lda, const float* sa, long l
     if (K <= 0) return AIEN_E_SHAPE;
     const F8Scales sc{sa, lds, sw, ldsw};
     AIEN_DISPATCH_DTYPE(c_dt, TC, return (launch_float8<TC>(a, lda, w, ldw, sc, out, ldc, M, N, K, w_ready, stream)));
+}
+
+// The product with act(gate) * up of its columns in 8 bits as its result: W's rows are gate and up in runs of 8 (N counts both), codes [M, N / 2], rows ldq
+// bytes apart, scales [ceil(N / 256), M], lds8 numbers apart.  In pairs of CTAs; rows of codes on 16-byte borders.
+AIEN_API int aien_matmul_swiglu_float8(const void* a, long lda, const float* sa, long lds, const void* w, long ldw, const float* sw, long ldsw,
+                                       void* codes, long ldq, float* scales, long lds8, int gelu, int M, int N, int K, cudaStream_t stream) {
+    using namespace aien;
+    if (M <= 0 || N <= 0) return 0;
+    if (K <= 0 || (N & 15)) return AIEN_E_SHAPE;
+    if (!f8_whole_rows(a, lda, w, ldw, M, N)) return AIEN_E_ALIGN;
+    return launch_float8_tiles<true, false, true, __nv_bfloat16>(a, lda, w, ldw, F8Scales{sa, lds, sw, ldsw}, nullptr, 0, M, N, K,
+                                                                 F8Gated8{(uint8_t*)codes, ldq, scales, lds8, gelu}, stream);
+}
+
+// Whether that is the product's own form at this size, so that one kernel takes less than two.
+AIEN_API int aien_matmul_swiglu_float8_supports(int M, int N, int K) {
+    return M > 0 && N > 0 && K > 0 && N % 16 == 0 && aien::f8_plan(M, N, K).form == 2;
 }

@@ -2619,3 +2619,31 @@ def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_sc
         _explain(name, ("out", out, (M, N), _F32_BF16), ("a", a, (M, width), _E4M3), ("a_scales", a_scales, (blocks, M), _F32), ("w", w, (N, width), _E4M3),
                  ("w_scales", w_scales, (n_blocks, blocks), _F32))
     _check(lib().aien_matmul_float8(a, lda, a_scales, ldsa, w, ldw, w_scales, ldsw, out, dt(out), ldo, M, N, width, 1 if w_ready else 0, _stream()), name)
+
+
+def matmul_swiglu_float8_pays(M: int, N: int, K_: int) -> bool:
+    """Whether :func:`matmul_swiglu_float8` takes less time than :func:`matmul_float8` and :func:`swiglu_float8`: where the product's own form at this size
+    is the one in pairs of CTAs."""
+    return bool(lib().aien_matmul_swiglu_float8_supports(int(M), int(N), int(K_)))
+
+
+def matmul_swiglu_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                         act: str = "silu") -> None:
+    """act(gate) * up of the product's columns in 8 bits, in the product's epilogue: the rows of w [2I, K] are gate and up interleaved in runs of 8 (I a
+    multiple of 8), codes [M, I], scales [ceil(I / 128), M].  gate and up are float32 here (the two kernels round them to 16 bits between).  Rows of a and w
+    start on 16-byte borders."""
+    name = "matmul_swiglu_float8"
+    M, I = _two(name, codes)
+    width = _two(name, a)[1]
+    blocks, n_blocks, o_blocks = float8_blocks(width), float8_blocks(2 * I), float8_blocks(I)
+    if act not in GATED_ACTS:
+        _refuse(name, f"activation {act!r}: known are {sorted(GATED_ACTS)}")
+    if I % 8:
+        _refuse(name, f"{I} columns do not divide into runs of 8")
+    lda, ldsa, ldw = _matrix(a, M, width, 4), _matrix(a_scales, blocks, M, 1), _matrix(w, 2 * I, width, 4)
+    ldsw, ldc, lds = _matrix(w_scales, n_blocks, blocks, 1), _matrix(codes, M, I, 4), _matrix(scales, o_blocks, M, 1)
+    if lda < 0 or ldsa < 0 or ldw < 0 or ldsw < 0 or ldc < 0 or lds < 0:
+        _explain(name, ("codes", codes, (M, I), _E4M3), ("scales", scales, (o_blocks, M), _F32), ("a", a, (M, width), _E4M3),
+                 ("a_scales", a_scales, (blocks, M), _F32), ("w", w, (2 * I, width), _E4M3), ("w_scales", w_scales, (n_blocks, blocks), _F32))
+    _check(lib().aien_matmul_swiglu_float8(a, lda, a_scales, ldsa, w, ldw, w_scales, ldsw, codes, ldc, scales, lds, 1 if act == "gelu_tanh" else 0,
+                                           M, 2 * I, width, _stream()), name)

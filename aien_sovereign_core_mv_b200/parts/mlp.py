@@ -17,8 +17,8 @@ class SwiGLU(FeedForward):
     transformer_backend.rs:1322-1362, silu in src/backend.rs:572-579).  gate and up are one
     product over the stacked rows gate | up (src/resident.rs:284-288).
 
-    ``weights`` "float8": h comes in 8 bits, both matrices are kept and multiplied in 8 bits, and so is what lies between them (act(gate) * up is
-    float32 of the first product's bfloat16 result)."""
+    ``weights`` "float8": h comes in 8 bits, both matrices are kept and multiplied in 8 bits, and so is what lies between them (act(gate) * up in
+    float32, of the first product's columns in its epilogue where rows are many, else of its bfloat16 result)."""
 
     offers_float8 = True
 
@@ -78,9 +78,12 @@ class SwiGLU(FeedForward):
 
     def forward(self, ctx: StepContext, h, sink: Optional[ResidualSink] = None):
         if self.takes_float8:
-            gu = linear_float8(ctx, h, self.w_gate_up)
-            rows = Float8Rows.take(ctx, gu.shape[0], self.intermediate_size)
-            K.swiglu_float8(gu, rows.codes, rows.scales, self.group, self.act)
+            T, w = h.codes.shape[0], self.w_gate_up
+            rows = Float8Rows.take(ctx, T, self.intermediate_size)
+            if self.group == 8 and K.matmul_swiglu_float8_pays(T, 2 * self.intermediate_size, self.hidden_size):
+                K.matmul_swiglu_float8(h.codes, h.scales, w.codes, w.scales, rows.codes, rows.scales, self.act)
+            else:
+                K.swiglu_float8(linear_float8(ctx, h, w), rows.codes, rows.scales, self.group, self.act)
             return linear_float8(ctx, rows, self.w_down)
         if isinstance(h, Prenormed):
             act = linear_prenormed(ctx, h, self.w_gate_up, epilogue=1) if self.group == 8 and self.act == "silu" else None

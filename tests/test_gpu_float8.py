@@ -259,6 +259,69 @@ def test_one_bad_number_stays_in_its_row(K, M):
     assert bool(torch.isnan(got[r]).all()) and torch.equal(got[:r], want[:r])
 
 
+def gated64(y, width, act):
+    """act(gate) * up of columns in runs of 8, and gate * up."""
+    v = y.view(y.shape[0], width // 8, 2, 8)
+    g, u = v[:, :, 0].reshape(-1, width), v[:, :, 1].reshape(-1, width)
+    z = math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)
+    return (g * torch.sigmoid(g) if act == "silu" else 0.5 * g * (1 + torch.tanh(z))) * u, g, u
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("M,I,width", [(1, 8, 16), (3, 136, 144), (130, 64, 128), (257, 264, 400), (300, 1000, 1040), (512, 1288, 640), (1500, 3200, 272)])
+@pytest.mark.parametrize("gap", [0, 1, 16])
+def test_gated_product(K, act, M, I, width, gap):
+    pad = -width % 16
+    a, w = codes_of(M, M, width, pad), codes_of(I, 2 * I, width, pad)
+    b, nb, ob = K.float8_blocks(width), K.float8_blocks(2 * I), K.float8_blocks(I)
+    # scales that bring the columns to about one: codes are 100 in the mean square, their products' sum 1e4 * sqrt(width)
+    sa, sw = scales_of(3, b, M) * 2.0 ** -6, scales_of(4, nb, b) * (2.0 ** -7 / width ** 0.5)
+    whole = torch.zeros(M, I + gap, dtype=torch.uint8, device="cuda").view(E4M3)
+    scales = torch.full((ob, M + gap), 7.0, device="cuda")
+    K.matmul_swiglu_float8(a, sa, w, sw, whole[:, :I], scales[:, :M], act=act)
+    want, total = product64(a, sa, w, sw)
+    y, g, u = gated64(want, I, act)
+    _, tg, tu = gated64(total, I, act)
+    # the columns are off by their sums' roundings (check_product); the activation passes an error of its argument on times at most 1.13 (both
+    # derivatives stay below that), its own value is off by 64 units of gate * up as in test_gated, or 1.2 |g| units more for |g| beyond 18
+    e = (128 + b + 3) * U
+    off = 1.13 * tg * e * (u.abs() + tu * e) + g.abs() * tu * e + (g * u).abs() * (64 + 1.2 * g.abs()) * U
+    check_scales(scales[:, :M].double().t(), y, off)
+    check_codes(whole[:, :I], scales[:, :M].double().t(), y, off)
+    assert bool((whole.view(torch.uint8)[:, I:] == 0).all()) and bool((scales[:, M:] == 7.0).all())
+    assert K.read_wait_errors() == (0, 0, 0, 0)
+
+
+def test_gated_product_of_bad_rows(K):
+    M, I, width = 300, 200, 256
+    a, w = codes_of(1, M, width).clone(), codes_of(2, 2 * I, width)
+    sa, sw = scales_of(3, 2, M) * 2.0 ** -12, scales_of(4, 4, 2) * 2.0 ** -8
+    e = lambda: (torch.empty(M, I, dtype=torch.uint8, device="cuda").view(E4M3), torch.empty(2, M, device="cuda"))
+    codes, scales = e()
+    K.matmul_swiglu_float8(a, sa, w, sw, codes, scales)
+    a.view(torch.uint8)[77, 3] = 0x7f
+    a.view(torch.uint8)[78] = 0
+    bad, bad_scales = e()
+    K.matmul_swiglu_float8(a, sa, w, sw, bad, bad_scales)
+    assert bool(torch.isnan(bad[77].float()).all()) and bool(torch.isnan(bad_scales[:, 77]).all())
+    assert bool((bad[78].float() == 0).all()) and bool((bad_scales[:, 78] == LEAST).all())
+    rest = [r for r in range(M) if r not in (77, 78)]
+    assert torch.equal(bad.view(torch.uint8)[rest], codes.view(torch.uint8)[rest]) and torch.equal(bad_scales[:, rest], scales[:, rest])
+
+
+def test_gated_product_refusals(K):
+    a, sa = codes_of(1, 5, 256), scales_of(2, 2, 5)
+    out = lambda I: (torch.empty(5, I, dtype=torch.uint8, device="cuda").view(E4M3), torch.empty(K.float8_blocks(I), 5, device="cuda"))
+    with pytest.raises(K.KernelError, match="runs of 8"):
+        K.matmul_swiglu_float8(a, sa, codes_of(3, 40, 256), scales_of(4, 1, 2), *out(20))
+    with pytest.raises(K.KernelError, match="activation 'relu'"):
+        K.matmul_swiglu_float8(a, sa, codes_of(3, 48, 256), scales_of(4, 1, 2), *out(24), act="relu")
+    with pytest.raises(K.KernelError, match="w has shape"):
+        K.matmul_swiglu_float8(a, sa, codes_of(3, 40, 256), scales_of(4, 1, 2), *out(24))
+    with pytest.raises(K.KernelError, match="aligned"):
+        K.matmul_swiglu_float8(codes_of(1, 5, 250), sa, codes_of(3, 48, 250), scales_of(4, 1, 2), *out(24))
+
+
 def test_nothing_to_do(K):
     w, sw = codes_of(1, 5, 200), scales_of(2, 1, 2)
     e = lambda *s: torch.empty(*s, dtype=torch.uint8, device="cuda").view(E4M3)
