@@ -39,7 +39,7 @@ inline bool f8_make_map_out(CUtensorMap* map, const void* ptr, uint64_t rows, ui
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {ld * sizeof(TC)};
+    cuuint64_t strides[1] = {rows > 1 ? ld * sizeof(TC) : (cols * sizeof(TC) + 15) / 16 * 16};
     cuuint32_t box[2] = {(cuuint32_t)(128 / sizeof(TC)), 32};
     cuuint32_t estr[2] = {1, 1};
     return fn(map, sizeof(TC) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, box, estr,
@@ -92,6 +92,13 @@ template <int N> struct F8Ring {
         if (++at == N) { at = 0; parity ^= 1; }
     }
 };
+
+// Waits until the last rounds of a ring of stages have been multiplied: every arrival at its barriers is then behind, and the CTA may leave.  A stage that
+// was never used passes at once, as it does in its first round.
+template <int N>
+__device__ __forceinline__ void f8_drain(uint32_t empty0, F8Ring<N> r) {
+    for (int i = 0; i < N; ++i, r.next()) mbar_wait(empty0 + 8 * r.at, r.parity ^ 1, 1);
+}
 
 __device__ __forceinline__ bool f8_try_wait_cluster(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -193,6 +200,7 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
             __syncwarp();
         }
+        f8_drain(empty0, r);
     } else if (warp == 1) {
         const uint32_t idesc = umma_idesc_e4m3(128, NT);
         const uint64_t dw0 = make_desc_sw128(sW), da0 = make_desc_sw128(sA);
@@ -352,27 +360,15 @@ __device__ __forceinline__ void f8_add_block(uint32_t taddr, float f, float (&ac
 
 // A warp's 32 rows x W columns of the result, a row a lane.  By TMA (the result's rows start on 16-byte borders): 128 bytes of a row at a time into
 // a buffer of 4 KB, 16-byte pieces swizzled as the copy expects them; rows and columns beyond the matrix are clipped by it.
-// Stored from registers each lane's 16 bytes are a row of their own (a tile of 128 x 256 took 6,700 cycles so).
+// Other results leave the buffer row after row.  Stored from registers each lane's 16 bytes are a row of their own (a tile of 128 x 256 took 6,700 cycles so).
 constexpr int F8_STORE = 4096;
 template <int W, typename TC>
 __device__ __forceinline__ void f8_store_rows(const float (&acc)[W], const CUtensorMap* map, bool by_tma, uint32_t at, TC* out, long ldc, int m, int n, int M, int N) {
     const int lane = threadIdx.x & 31;
-    if (!by_tma) {
-        if (m + lane < M) {
-#pragma unroll
-            for (int c0 = 0; c0 < W; c0 += 32) {
-                uint32_t r[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(acc[c0 + j]);
-                if (n + c0 < N) tc_store_chunk<0, TC>(r, out, ldc, m + lane, n, c0, N);
-            }
-        }
-        return;
-    }
     constexpr int COLS = 128 / sizeof(TC);
 #pragma unroll
     for (int c0 = 0; c0 < W; c0 += COLS) {
-        if (lane == 0) tma_store_read<0>();                                   // the last copy has read the buffer
+        if (by_tma && lane == 0) tma_store_read<0>();                         // the last copy has read the buffer
         __syncwarp();
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
@@ -390,11 +386,34 @@ __device__ __forceinline__ void f8_store_rows(const float (&acc)[W], const CUten
             }
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 128 + ((p ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-            if (m < M && n + c0 < N) tma_store_2d(at, map, n + c0, m);
-            tma_store_commit();
+        if (by_tma) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (m < M && n + c0 < N) tma_store_2d(at, map, n + c0, m);
+                tma_store_commit();
+            }
+        } else {                                                              // row after row, neighbouring lanes neighbouring numbers
+            __syncwarp();
+            const int end = min(32, M - m);
+#pragma unroll 4
+            for (int r = 0; r < end; ++r) {
+                TC* to = out + (long)(m + r) * ldc + n + c0;
+#pragma unroll
+                for (int c = lane; c < COLS; c += 32) {
+                    const uint32_t from = at + r * 128 + ((((uint32_t)c * (uint32_t)sizeof(TC)) >> 4 ^ (r & 7)) << 4) + (c * sizeof(TC) & 15);
+                    TC v;
+                    if constexpr (sizeof(TC) == 2) {
+                        uint16_t h;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from) : "memory");
+                        v = __ushort_as_bfloat16(h);
+                    } else {
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
+                    }
+                    if (n + c0 + c < N) to[c] = v;
+                }
+            }
+            __syncwarp();
         }
     }
 }
@@ -403,59 +422,97 @@ __device__ __forceinline__ void f8_store_rows(const float (&acc)[W], const CUten
 // and the sums of its own rows in its tensor memory; the first issues the instructions for both.  Alone, a CTA makes 128 x 128.
 // Shared memory is what the tensor cores wait for next: per k-block of 128 x 256 sums an SM's take 64 KB out of it in a pair and 96 alone, 128 as two
 // of 128 x 128, beside the 32, 48 or 64 that TMA puts in, at 128 bytes a cycle, while the sums take 512 cycles.
-template <bool PAIR> struct F8Tiles {
+constexpr int F8_RAW_ROW = 144, F8_RAW = 256 * F8_RAW_ROW, F8_RAWS = 3;                   // rows as they lie in memory: a k-block's, so many of them
+// GATHER: the ring is two stages, the rest of its room the rows as they lie in memory.
+template <bool PAIR, bool GATHER> struct F8Tiles {
     static constexpr int P = PAIR ? 2 : 1, BM = 128 * P, BN = 128 * P;
-    static constexpr int STAGE_A = 128 * F8_KB, STAGE_W = 128 * F8_KB, STAGES = 5;
+    static constexpr int STAGE_A = 128 * F8_KB, STAGE_W = 128 * F8_KB, STAGES = GATHER ? 2 : 5;
     static constexpr int BUFS = 512 / BN;
-    static constexpr int RING = STAGES * (STAGE_A + STAGE_W), STORES = 8 * F8_STORE;
-    static constexpr int SMEM = RING + STORES + F8_SLOTS * F8_SLOT + 1024 /*align*/ + 256 /*barriers*/;
+    static constexpr int RING = STAGES * (STAGE_A + STAGE_W), STORES = 8 * F8_STORE, RAWS = GATHER ? F8_RAWS * F8_RAW : 0;
+    static constexpr int SMEM = RING + RAWS + STORES + F8_SLOTS * F8_SLOT + 1024 /*align*/ + 256 /*barriers*/;
     static_assert(SMEM <= 227 * 1024, "a CTA's shared memory");
 };
 
-// Rows of codes that start anywhere, which TMA does not take: 128 threads bring a tile's 128 rows x 128 codes, each 16 codes of eight rows, in aligned words that
-// are shifted into place, and put them where TMA would.  A word that reaches over an end of the row is put together from its bytes within it, so that
-// nothing outside the rows is read; codes beyond the row and rows beyond the matrix are zeros.  Twenty words of each thread are on their way at a time.
-__device__ __forceinline__ uint32_t f8_word(const uint8_t* word, const uint8_t* begin, const uint8_t* end) {
-    if (word >= begin && word + 4 <= end) return __ldcg(reinterpret_cast<const uint32_t*>(word));
-    uint32_t v = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (word + i >= begin && word + i < end) v |= (uint32_t)__ldcg(word + i) << (8 * i);
-    return v;
-}
-__device__ __forceinline__ void f8_gather(uint32_t tile, const uint8_t* p, long ld, int row0, int rows, int k0, int K, int thread) {
-    const int chunk = thread & 7;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        uint32_t v[4][5];
-        uint32_t shift[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = row0 + (thread >> 3) + (half * 4 + i) * 16;
-            const uint8_t* begin = p + (r < rows ? (long)r * ld : 0);
-            const uint8_t* end = begin + (r < rows ? K : 0);
-            const uint8_t* from = begin + k0 + chunk * 16;
-            const uint8_t* word = reinterpret_cast<const uint8_t*>((uintptr_t)from & ~(uintptr_t)3);
-            shift[i] = ((uint32_t)(uintptr_t)from & 3) * 8;
-#pragma unroll
-            for (int j = 0; j < 5; ++j) v[i][j] = f8_word(word + 4 * j, begin, end);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (thread >> 3) + (half * 4 + i) * 16;
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(v[i][j], v[i][j + 1], shift[i]);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + r * 128 + ((chunk ^ (r & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-        }
-    }
-}
+// Rows of codes that start anywhere, which TMA does not take: 128 threads bring a k-block of a tile's 128 + 128 rows.  First as it lies in memory, in the nine
+// 16-byte words that the 128 codes of a row touch, asynchronously and two k-blocks ahead; then shifted into place, where TMA would have put it.  Codes
+// beyond a row and rows beyond the matrix become zeros.  Nothing outside the matrix is read: the copy of a word stops at its row's end, and the
+// one word that may begin before the matrix is put together from its bytes.
 struct F8Rows {
     const uint8_t* a;
     long lda;
     const uint8_t* w;
     long ldw;
 };
+// What a thread copies of a tile: word 16 * (thread + 128 i) of the k-block's 256 rows of nine, from its place in the first k-block on; how many codes of its row
+// lie behind its beginning.
+struct F8Words {
+    const uint8_t* word[18];
+    int left[18];
+    __device__ __forceinline__ void start(const F8Rows& t, int m0, int M, int n0, int N, int K, int thread) {
+        int row = thread / 9, c = thread % 9;
+#pragma unroll
+        for (int i = 0; i < 18; ++i) {
+            const int r = row < 128 ? m0 + row : n0 + row - 128;
+            const bool live = r < (row < 128 ? M : N);
+            const uint8_t* begin = row < 128 ? t.a + (live ? (long)r * t.lda : 0) : t.w + (live ? (long)r * t.ldw : 0);
+            const uint32_t off = (uint32_t)(uintptr_t)begin & 15;
+            word[i] = begin - off + 16 * c;
+            left[i] = !live || (c == 8 && off == 0) ? -1 : (int)off + K - 16 * c;           // (the ninth word of a row that starts on a border is the next k-block's)
+            if (live) left[i] = max(left[i], -1);
+            row += 14;                                                        // 128 = 14 x 9 + 2
+            c += 2;
+            if (c >= 9) { c -= 9; ++row; }
+        }
+    }
+    // k-block kb's into the raw rows at `raw`
+    __device__ __forceinline__ void copy(uint32_t raw, const F8Rows& t, int kb, int thread) const {
+#pragma unroll
+        for (int i = 0; i < 18; ++i) {
+            const uint8_t* from = word[i] + (long)kb * F8_KB;
+            const int bytes = min(max(left[i] - kb * F8_KB, 0), 16);
+            const uint32_t dst = raw + 16 * (thread + 128 * i);
+            if ((i == 0 || i == 9) && from < (i == 0 ? t.a : t.w) && bytes > 0) {           // thread 0, the matrix' first word: it begins before the matrix
+                uint32_t v[4] = {0, 0, 0, 0};
+                for (int b = 0; b < 16; ++b)
+                    if (from + b >= (i == 0 ? t.a : t.w) && b < bytes) v[b >> 2] |= (uint32_t)__ldcg(from + b) << (8 * (b & 3));
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+            } else {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(bytes > 0 ? from : word[i]), "r"(bytes) : "memory");
+            }
+        }
+    }
+};
+// How far a thread's sixteen rows ((thread / 8) + 16 i of the tile's 256) start behind a border, four bits each.
+__device__ __forceinline__ uint64_t f8_offsets(const F8Rows& t, int m0, int n0, int thread) {
+    uint64_t packed = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = (thread >> 3) + i * 16;
+        const uint8_t* p = row < 128 ? t.a + (long)(m0 + row) * t.lda : t.w + (long)(n0 + row - 128) * t.ldw;
+        packed |= (uint64_t)((uintptr_t)p & 15) << (4 * i);
+    }
+    return packed;
+}
+// 16 codes of each of those rows, chunk thread % 8, from the raw rows to where TMA would have put them
+__device__ __forceinline__ void f8_place_raw(uint32_t raw, uint32_t tile_a, uint32_t tile_w, uint64_t offsets, int thread) {
+    const int chunk = thread & 7, first = thread >> 3;
+    const uint32_t from = raw + first * F8_RAW_ROW + chunk * 16, to = first * 128 + ((chunk ^ (first & 7)) << 4);
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t s = (uint32_t)(offsets >> (4 * i)) & 15, at = from + i * (16 * F8_RAW_ROW);
+        uint32_t v[8];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(at + 16) : "memory");
+#pragma unroll
+        for (int j = 0; j < 6; ++j) v[j] = s & 8 ? v[j + 2] : v[j];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) v[j] = s & 4 ? v[j + 1] : v[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __funnelshift_r(v[j], v[j + 1], (s & 3) * 8);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((i < 8 ? tile_a + to + i * 2048 : tile_w + to + (i - 8) * 2048)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                     "r"(v[3]) : "memory");
+    }
+}
 
 // Where a gated product's result goes: codes [M, N / 2] and scales [ceil(N / 256), M].
 struct F8Gated8 {
@@ -509,12 +566,12 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     int store_by_tma, F8Scales sc, TC* __restrict__ out, long ldc, int M, int N, int K, int m_tiles, int tiles, F8Rows rows, F8Gated8 gated) {
     static_assert(!(PAIR && GATHER), "rows that start anywhere are multiplied in tiles of one CTA");
     static_assert(PAIR || !GATED, "a block of a gated result is 256 columns");
-    using C = F8Tiles<PAIR>;
+    using C = F8Tiles<PAIR, GATHER>;
     constexpr int P = C::P;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t sA = base, sW = base + C::STAGES * C::STAGE_A, sStore = base + C::RING, sScale = sStore + C::STORES;
+    const uint32_t sA = base, sW = base + C::STAGES * C::STAGE_A, sRaw = base + C::RING, sStore = sRaw + C::RAWS, sScale = sStore + C::STORES;
     const uint32_t bars = sScale + F8_SLOTS * F8_SLOT;
     const uint32_t full0 = bars, empty0 = full0 + 8 * C::STAGES, tfull0 = empty0 + 8 * C::STAGES, tempty0 = tfull0 + 8 * C::BUFS;
     const uint32_t sfull0 = tempty0 + 8 * C::BUFS, sempty0 = sfull0 + 8 * F8_SLOTS, slot = sempty0 + 8 * F8_SLOTS;
@@ -571,6 +628,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     __syncwarp();
                 }
             }
+            f8_drain(empty0, r);
         } else if (warp == 1 && rank == 0) {
             const uint32_t idesc = umma_idesc_e4m3(C::BM, C::BN);
             const uint64_t da0 = make_desc_sw128(sA), dw0 = make_desc_sw128(sW);
@@ -623,16 +681,34 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         griddep_wait();
         const int thread = threadIdx.x - 384;
         F8Ring<C::STAGES> r;
+        F8Ring<F8_RAWS> in, have;
+        int ptile = first, pkb = 0;                                           // two k-blocks ahead
+        F8Words words;
+        auto request = [&]() {
+            if (ptile < tiles) {
+                if (pkb == 0) words.start(rows, ptile % m_tiles * C::BM, M, ptile / m_tiles * C::BN, N, K, thread);
+                words.copy(sRaw + in.at * F8_RAW, rows, pkb, thread);
+                in.next();
+                if (++pkb == blocks) { pkb = 0; ptile += step; }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        request();
+        request();
         for (int tile = first; tile < tiles; tile += step) {
-            const int m0 = tile % m_tiles * C::BM, n0 = tile / m_tiles * C::BN;
-            for (int kb = 0; kb < blocks; ++kb, r.next()) {
+            const uint64_t offsets = f8_offsets(rows, tile % m_tiles * C::BM, tile / m_tiles * C::BN, thread);
+            for (int kb = 0; kb < blocks; ++kb, r.next(), have.next()) {
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                asm volatile("bar.sync 3, 128;" ::: "memory");                // everyone's copies of this k-block are there, and everyone is through with the one before
+                request();
                 mbar_wait(empty0 + 8 * r.at, r.parity ^ 1, 1);
-                f8_gather(sA + r.at * C::STAGE_A, rows.a, rows.lda, m0, M, kb * F8_KB, K, thread);
-                f8_gather(sW + r.at * C::STAGE_W, rows.w, rows.ldw, n0, N, kb * F8_KB, K, thread);
+                f8_place_raw(sRaw + have.at * F8_RAW, sA + r.at * C::STAGE_A, sW + r.at * C::STAGE_W, offsets, thread);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(full0 + 8 * r.at);
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        f8_drain(empty0, r);
     } else {
         // (the shares add up to what the CTA was launched with: 40 + 2 x 232 = 3 x 168, with four warps more 40 + 120 + 2 x 176 = 4 x 128)
         if (GATHER) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
@@ -730,7 +806,8 @@ inline int f8_launch(void (*kernel)(KArgs...), dim3 grid, int threads, int smem,
     cfg.attrs = attr;
     cfg.numAttrs = n;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-    return e != cudaSuccess ? (int)e : launch_status();
+    const int status = launch_status();                                       // (a failed launch leaves nothing behind for the next one to report)
+    return e != cudaSuccess ? (int)e : status;
 }
 
 inline int f8_sms() {
@@ -752,7 +829,7 @@ int launch_float8_few(const void* a, long lda, const void* w, long ldw, F8Scales
 
 template <bool PAIR, bool GATHER, bool GATED, typename TC>
 int launch_float8_tiles(const void* a, long lda, const void* w, long ldw, F8Scales sc, void* out, long ldc, int M, int N, int K, F8Gated8 gated, cudaStream_t stream) {
-    using C = F8Tiles<PAIR>;
+    using C = F8Tiles<PAIR, GATHER>;
     constexpr int P = C::P;
     CUtensorMap ma = {}, mw = {}, mo = {};
     if (!GATHER && (!f8_make_map(&ma, a, M, K, lda, 128) || !f8_make_map(&mw, w, N, K, ldw, 128))) return AIEN_E_STATE;
@@ -789,6 +866,7 @@ inline F8Plan f8_plan(int M, int N, int K) {
         const double t = (Z == 1 ? 2.3 : 4.0) + (double)((blocks + Z - 1) / Z) * each * (double)((ctas + 2 * sms - 1) / (2 * sms));
         if (t < least) { least = t; best.Z = Z; }
     }
+    if (n_tiles > 65535) return F8Plan{1, 1};                                 // beyond the grid of the form for few rows
     if (M <= 64) return best;
     const long alone = ((long)M + 127) / 128 * n_tiles, pairs = ((long)M + 255) / 256 * (((long)N + 255) / 256);
     const double t1 = 3.2 + 0.28 * blocks * (double)((alone + sms - 1) / sms), t2 = 3.0 + 0.44 * blocks * (double)((pairs + sms / 2 - 1) / (sms / 2));

@@ -2603,7 +2603,8 @@ def quantize_blocks_float8(w: torch.Tensor, codes: torch.Tensor, scales: torch.T
 
 def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, w_ready: bool = False) -> None:
     """out [M, N] (bfloat16 or float32, row stride free) = a . w^T of rows a [M, K] with scales [ceil(K / 128), M] and a weight w [N, K] with scales
-    [ceil(N / 128), ceil(K / 128)]: a block's sum of code products times its two scales, the blocks added up in float32.
+    [ceil(N / 128), ceil(K / 128)]: a block's sum of code products times its two scales, the blocks added up in float32.  The two scales are
+    multiplied first: their product belongs in float32's range.
 
     ``w_ready``: w was written before the kernels that are unfinished in the stream were launched (a model's weights during a step), so that
     it may be requested ahead of their end."""

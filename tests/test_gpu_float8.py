@@ -201,7 +201,7 @@ def check_product(out, a, sa, w, sw):
     assert not bool((far > 0).any()), (float(far.max()), float(((out.double() - want).abs() / off).max()))
 
 
-PRODUCTS = [(1, 1, 1), (1, 128, 128), (1, 4096, 4096), (2, 130, 127), (3, 64, 129), (8, 1000, 2064), (16, 257, 4096), (17, 640, 256), (31, 129, 1000),
+PRODUCTS = [(1, 1, 1), (1, 130, 127), (1, 1000, 1001), (1, 128, 128), (2, 1, 300), (1, 4096, 4096), (2, 130, 127), (3, 64, 129), (8, 1000, 2064), (16, 257, 4096), (17, 640, 256), (31, 129, 1000),
             (33, 520, 12288), (64, 300, 1008), (65, 384, 384), (100, 96, 144), (127, 1000, 512), (128, 128, 640), (129, 257, 272), (200, 1040, 1040),
             (256, 512, 2048), (300, 2000, 400), (513, 777, 1111), (1030, 1100, 1552), (2048, 1536, 512)]
 
@@ -237,6 +237,26 @@ def test_product_starts_anywhere(K, M):
     a, w = codes_of(1, M, width + 40)[:, 13:13 + width], codes_of(2, N, width + 21)[:, 5:5 + width]
     sa, sw = scales_of(3, 3, M + 1)[:, 1:], scales_of(4, 3, 4)[:, 1:]
     out = torch.empty(M, N + 1, device="cuda")[:, 1:]
+    K.matmul_float8(a, sa, w, sw, out)
+    check_product(out, a, sa, w, sw)
+
+
+@pytest.mark.parametrize("at,gap", [(0, 16), (16, 32), (1, 3), (15, 0), (5, 11)])
+@pytest.mark.parametrize("M,N,width", [(1, 130, 120), (20, 130, 129), (100, 200, 1000), (300, 260, 257), (600, 1030, 400)])
+def test_what_lies_around_the_rows_is_not_looked_at(K, M, N, width, at, gap):
+    """Codes that are not numbers before, between and behind the rows; scales that are not numbers beside the ones that count."""
+    ld = width + at + gap
+    def among_nan(seed, rows):
+        whole = torch.full((rows + 2, ld), 0x7f, dtype=torch.uint8, device="cuda").view(E4M3)
+        part = whole[1:rows + 1, at:at + width]
+        part.view(torch.uint8).copy_(codes_of(seed, rows, width).view(torch.uint8))
+        return part
+    a, w = among_nan(1, M), among_nan(2, N)
+    b, nb = K.float8_blocks(width), K.float8_blocks(N)
+    sa, sw = torch.full((b + 1, M + 3), math.nan, device="cuda"), torch.full((nb + 1, b + 2), math.nan, device="cuda")
+    sa[:b, 2:2 + M], sw[:nb, 1:1 + b] = scales_of(3, b, M), scales_of(4, nb, b)
+    sa, sw = sa[:b, 2:2 + M], sw[:nb, 1:1 + b]
+    out = torch.empty(M, N, device="cuda")
     K.matmul_float8(a, sa, w, sw, out)
     check_product(out, a, sa, w, sw)
 
@@ -350,12 +370,12 @@ class Layer:
         self.K.quantize_blocks_float8(self.raw_up, self.up, self.up_s)
         self.K.quantize_blocks_float8(self.raw_down, self.down, self.down_s)
 
-    def step(self, x, delta):
+    def step(self, x, delta, w_ready=False):
         K = self.K
         K.add_rmsnorm_float8(x, delta, self.norm, 1e-6, self.h, self.h_s)
-        K.matmul_float8(self.h, self.h_s, self.up, self.up_s, self.gu)
+        K.matmul_float8(self.h, self.h_s, self.up, self.up_s, self.gu, w_ready=w_ready)
         K.swiglu_float8(self.gu, self.act, self.act_s, group=8)
-        K.matmul_float8(self.act, self.act_s, self.down, self.down_s, self.y)
+        K.matmul_float8(self.act, self.act_s, self.down, self.down_s, self.y, w_ready=w_ready)
         return self.y
 
 
@@ -381,10 +401,11 @@ def test_a_layer_of_them(K, T, H, I):
     g = (h @ m.raw_up.double().t()).view(T, I // 8, 2, 8)
     want = (g[:, :, 0] * torch.sigmoid(g[:, :, 0]) * g[:, :, 1]).reshape(T, I) @ m.raw_down.double().t()
     assert float((y.double() - want).norm() / want.norm()) < 4 * 2.0 ** -4 / 3 * 2
-    for _ in range(20):
-        m.weights()
+    for i in range(20):
+        if i < 10:
+            m.weights()
         x.copy_(x0)
-        m.step(x, delta)
+        m.step(x, delta, w_ready=i >= 10)                # the weights stay as they are from here on
     assert torch.equal(m.y, y)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
