@@ -12,7 +12,21 @@ __device__ __forceinline__ uint32_t f8_bits(float v) { return __float_as_uint(fa
 __device__ __forceinline__ float f8_scale(uint32_t top) {
     return top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(top) * (1.0f / F8_TOP), F8_LEAST);
 }
-__device__ __forceinline__ float f8_inverse(float scale) { return __frcp_rn(scale); }
+// One instruction of the special-function unit, at most a unit off; a scale and its reciprocal are ordinary numbers (2^-126 to 2^120).
+__device__ __forceinline__ float f8_reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float f8_inverse(float scale) { return f8_reciprocal(scale); }
+// act(g) * u: silu, or the gelu in its tanh form, from one exponential and one reciprocal (for large -g the exponential is infinite, its reciprocal 0).
+template <bool GELU>
+__device__ __forceinline__ float f8_gate(float g, float u) {
+    if (GELU) return 0.5f * g * (1.0f + tanh_ex2(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
+    float t;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -1.4426950408889634f));
+    return g * f8_reciprocal(1.0f + t) * u;
+}
 __device__ __forceinline__ uint32_t f8_pair(float a, float b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }

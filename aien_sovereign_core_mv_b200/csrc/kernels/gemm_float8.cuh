@@ -531,8 +531,7 @@ __device__ __forceinline__ void f8_store_gated(float (&acc)[128], const F8Gated8
     for (int v = 0; v < 8; ++v)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float z = acc[16 * v + j], u = acc[16 * v + 8 + j];
-            const float y = (g.gelu ? 0.5f * z * (1.0f + tanh_ex2(0.7978845608028654f * (z + 0.044715f * z * z * z))) : __fdividef(z, 1.0f + __expf(-z))) * u;
+            const float y = g.gelu ? f8_gate<true>(acc[16 * v + j], acc[16 * v + 8 + j]) : f8_gate<false>(acc[16 * v + j], acc[16 * v + 8 + j]);
             acc[8 * v + j] = y;
             if (n + 16 * v < N) top = max(top, f8_bits(y));
         }
