@@ -253,8 +253,8 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             f8_arrive0(tempty0 + 8 * t.at, lane);
         }
     }
-    const int n = n0 + row;
-    if (Z == 1) {
+    if (Z == 1) {                                                             // nobody to add to: straight from the registers
+        const int n = n0 + row;
         if (warp >= 2 && n < N) {
 #pragma unroll
             for (int i = 0; i < NT / 2; ++i) {
@@ -264,9 +264,8 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
         }
     } else {
-        // CTA z takes columns z * NT / Z .. of everyone's sums and adds them up in the order of K.  They lie by owner in the ring, whose
-        // last stage has been multiplied, [owner][column][row]; one copy a CTA brings them to [from][column][row] in the owner's place for them.
-        // (Stored over the cluster number by number they took 2 us.)
+        // The sums go into the ring, whose last stage has been multiplied, [column][row].  CTA z takes columns z * NT / Z .. of everyone's: one
+        // copy a CTA brings them to [from][column][row] in the owner's place for them (stored over the cluster number by number they took 2 us).
         const int cw = NT / Z;
         const uint32_t piece = C::PARTS / Z;
         if (warp >= 2) {
@@ -287,12 +286,35 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         __syncwarp();
         if (warp >= 2) f8_wait_cluster(parts_in, 0, 3);
         asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); // what others sent has arrived: when everyone says so, everyone may leave
-        if (warp >= 2 && n < N) {
-            for (int c = 0; c < cw && m0 + rank * cw + c < M; ++c) {
-                float v = 0.f;
-                for (int z = 0; z < Z; ++z)
-                    v += reinterpret_cast<const volatile float*>(z == rank ? gen + z * piece : gen + (sParts - base) + z * piece)[c * 128 + row];
-                out[(long)(m0 + rank * cw + c) * ldc + n] = from_f<TC>(v);
+        if (warp >= 2) {
+            // Added up in the order of K.  Where two numbers make an aligned word, a thread takes two neighbours of every other column (one number of
+            // every column: 64 x 4,096 x 12,288 in 17.3 us for 16.2).
+            const bool two = (((uintptr_t)out | (uintptr_t)ldc * sizeof(TC)) & (2 * sizeof(TC) - 1)) == 0;
+            const int r = two ? 2 * (pt & 63) : pt, n = n0 + r, step = two ? 2 : 1;
+#pragma unroll 2
+            for (int c = two ? pt >> 6 : 0; c < cw; c += step) {
+                const int m = m0 + rank * cw + c;
+                float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int z = 0; z < 8; ++z) {
+                    if (z >= Z) break;
+                    const float* p = reinterpret_cast<const float*>((z == rank ? gen : gen + (sParts - base)) + z * piece) + c * 128 + r;
+                    if (two) {
+                        const float2 q = *reinterpret_cast<const float2*>(p);
+                        v.x += q.x;
+                        v.y += q.y;
+                    } else {
+                        v.x += *p;
+                    }
+                }
+                if (m >= M || n >= N) continue;
+                TC* to = out + (long)m * ldc + n;
+                if (two && n + 1 < N) {
+                    if constexpr (sizeof(TC) == 2) *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(v.x, v.y);
+                    else *reinterpret_cast<float2*>(to) = v;
+                } else {
+                    *to = from_f<TC>(v.x);
+                }
             }
         }
         __syncwarp();
