@@ -102,7 +102,7 @@ __device__ __forceinline__ void f8_store(uint8_t* codes, int k0, int lane, int K
 // Half a warp takes a block of a row, U blocks of it one after the other whose loads are all on their way first.  A CTA's 16 halves are `rows` rows times
 // 16 / rows neighbouring blocks (rows a power of two): one row where it has sixteen blocks, so that what a CTA reads lies together (gated, 512 x 12,288 in 7.6 us;
 // two rows of eight 7.8, eight rows of two, whose scales leave together, 8.1).
-// (As many CTAs as the GPU holds, walking over the blocks with the next one's numbers on their way, took longer: 2,048 x 12,288 gated in 37 us.)
+// (As many CTAs as the GPU holds, walking over the blocks with the next one's numbers on their way, took longer: 2,048 x 12,288 gated in 37 us for 31.)
 template <typename SRC, bool VEC, int U>
 __global__ void __launch_bounds__(256)
 rows_float8_kernel(SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, int rows) {
@@ -156,8 +156,8 @@ static int launch_rows_float8_by(SRC src, uint8_t* codes, long ldq, float* scale
     launch_chain(rows_float8_kernel<SRC, VEC, U>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, stream, src, codes, ldq, scales, lds, T, K, rows);
     return launch_status();
 }
-// Two blocks a half from two loads of the GPU on (148 SMs of 128 halves): gated, 2,048 x 12,288 in 31.4 us by one and 27.7 by two (by four 28.4), 512 x 12,288 in
-// 9.3 and 8.8, but 64 x 12,288 in 2.5 and 3.2; rows of 2,048 x 4,096 in 8.1 and 7.0, of 512 x 4,096 in 3.0 and 3.5.
+// Two blocks a half from two loads of the GPU on (148 SMs of 128 halves): gated, 2,048 x 12,288 in 26.4 us by one and 23.9 by two, 512 x 12,288 in 8.0 and
+// 7.6, but 64 x 12,288 in 2.3 and 2.7; rows of 2,048 x 4,096 in 7.3 and 6.2, of 512 x 4,096 in 3.0 and 3.2.
 template <typename SRC>
 static int launch_rows_float8(bool vec, SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, cudaStream_t stream) {
     if (!vec) return launch_rows_float8_by<SRC, false, 1>(src, codes, ldq, scales, lds, T, K, stream);

@@ -871,12 +871,13 @@ int launch_float8_tiles(const void* a, long lda, const void* w, long ldw, F8Scal
 // The product's form, by the time that each would take (us; measured with K of 4,096 and 12,288 on rows of 8 to 4,096, with one to three waves):
 //   in tiles of 128 x 128      3.2 and 0.28 a k-block and wave of one tile an SM
 //   in pairs, 256 x 256        3.0 and 0.44 a k-block and wave of one tile a pair of SMs
-//   few rows, 128 x NT         2.3, shared by a cluster of 2, 4 or 8 4.6, 3.7 or 4.1, with 64 columns 4 more, and a k-block 0.23 where the CTAs are few,
-//                              else W's bytes at 6.5 TB/s; more than 64 rows in tiles of 64 0.002 a CTA, which L2 and the reading of tensor memory
-//                              take; two CTAs an SM
-// 256 x 4,096 x 4,096: 11.8 us in tiles, 15.5 in pairs, 16.6 in the form for few rows; 128 x 4,096 x 12,288: 28.2, 37.0 and 18.2;
-// 1,024 x 4,096 x 4,096: 20.7, 17.1 and 36.8.  8 rows by clusters of 1, 2, 4 and 8: 4,096 x 4,096 9.7, 8.2, 6.2 and 6.6; 6,144 x 4,096 10.2, 9.1, 7.7 and
-// 10.4; 4,096 x 12,288 24.4, 15.5, 11.4 and 11.6; 24,576 x 4,096 19.6, 24.4, 23.2 and 31.7.
+//   few rows, 128 x NT         2.3, shared by a cluster of 2, 4 or 8 4.6, 3.7 or 4.1 (with 64 columns 2.2 more), and a k-block 0.23 where the CTAs are
+//                              few (with 64 columns, whose ring is shorter, 0.39), else W's bytes at 6.5 TB/s; more than 64 rows in tiles of 64
+//                              0.002 a CTA, which L2 and the reading of tensor memory take; two CTAs an SM
+// 256 x 4,096 x 4,096: 11.8 us in tiles, 15.5 in pairs, 16.6 in the form for few rows; 128 x 4,096 x 12,288: 28.2, 37.0 and 17.8;
+// 1,024 x 4,096 x 4,096: 20.7, 17.1 and 36.8; 67 x 1,000 x 2,064: 8.8 in tiles and 7.3 in the form for few rows.  8 rows by clusters of 1, 2, 4 and 8:
+// 4,096 x 4,096 9.7, 8.2, 6.2 and 6.6; 6,144 x 4,096 10.2, 9.1, 7.7 and 10.4; 4,096 x 12,288 24.4, 15.5, 11.4 and 11.6; 24,576 x 4,096 19.6, 24.4, 23.2
+// and 31.7.
 struct F8Plan {
     int form, Z;              // columns of the form for few rows (16, 32 or 64), 1 tiles, 2 pairs; CTAs that share K
 };
@@ -888,8 +889,8 @@ inline F8Plan f8_plan(int M, int N, int K) {
     double least = 1e30;
     for (int Z = 1; Z <= 8 && Z <= blocks; Z *= 2) {
         const long ctas = few * Z, at_once = ctas < 2 * sms ? ctas : 2 * sms;
-        const double busy = at_once * (M <= 64 ? 0.0025 : 0.002), each = busy > 0.23 ? busy : 0.23;
-        const double t = (Z == 1 ? 2.3 : Z == 2 ? 4.6 : Z == 4 ? 3.7 : 4.1) + (nt == 64 ? 4.0 : 0.) + (double)((blocks + Z - 1) / Z) * each * (double)((ctas + 2 * sms - 1) / (2 * sms));
+        const double busy = at_once * (M <= 64 ? 0.0025 : 0.002), least_each = nt == 64 ? 0.39 : 0.23, each = busy > least_each ? busy : least_each;
+        const double t = (Z == 1 ? 2.3 : Z == 2 ? 4.6 : Z == 4 ? 3.7 : 4.1) + (nt == 64 ? 2.2 : 0.) + (double)((blocks + Z - 1) / Z) * each * (double)((ctas + 2 * sms - 1) / (2 * sms));
         if (t < least) { least = t; best.Z = Z; }
     }
     if (n_tiles > 65535) return F8Plan{1, 1};                                 // beyond the grid of the form for few rows
