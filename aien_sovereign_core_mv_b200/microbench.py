@@ -6,6 +6,7 @@
     python -m aien_sovereign_core_mv_b200.microbench attn-prefill --tokens 2048 --impl tc
     python -m aien_sovereign_core_mv_b200.microbench qk --tokens 2048
     python -m aien_sovereign_core_mv_b200.microbench sample --rows 8 --top-p 0.95
+    python -m aien_sovereign_core_mv_b200.microbench float8 --m 8 --n 24576 --k 4096
     python -m aien_sovereign_core_mv_b200.microbench all
 
 Every case launches its kernel a few times eagerly (what a profiler captures) and then times a
@@ -50,6 +51,29 @@ def gemv_case(n: int, k: int, m: int, epilogue: int, reps: int = 20) -> None:
         K.gemv(a, ws[i % copies], out, epilogue=epilogue)
     us = _time_graph(lambda i: K.gemv(a, ws[i % copies], out, epilogue=epilogue), reps)
     print(f"gemv[{K.GEMV_IMPL}] N={n} K={k} M={m} epilogue={epilogue}: {us:8.2f} us  {n * k * 2 / us / 1e3:7.0f} GB/s of weights", flush=True)
+
+
+def float8_case(m: int, n: int, k: int, reps: int = 10) -> None:
+    """The product of m rows in 8 bits by a weight [n, k] in 8 bits, and the steps that leave such rows: the residual sum and norm of width k, the gated
+    activation of n / 2 columns."""
+    copies = max(2, int(1.5e9 // (n * k)))
+    E, b = torch.float8_e4m3fn, K.float8_blocks
+    empty = lambda *shape: torch.empty(*shape, device="cuda", dtype=torch.uint8).view(E)
+    scales = lambda *shape: torch.empty(*shape, device="cuda")
+    ws = []
+    for _ in range(copies):
+        ws.append((empty(n, k), scales(b(n), b(k))))
+        K.quantize_blocks_float8(torch.randn(n, k, device="cuda", dtype=torch.bfloat16), *ws[-1])
+    a, sa = empty(m, k), scales(b(k), m)
+    x, delta, norm = torch.randn(m, k, device="cuda"), torch.randn(m, k, device="cuda", dtype=torch.bfloat16), torch.ones(k, device="cuda")
+    out, act, s_act = torch.empty(m, n, device="cuda", dtype=torch.bfloat16), empty(m, n // 2), scales(b(n // 2), m)
+    steps = {"product": lambda i: K.matmul_float8(a, sa, *ws[i % copies], out), "norm": lambda i: K.add_rmsnorm_float8(x, delta, norm, 1e-6, a, sa),
+             "gated": lambda i: K.swiglu_float8(out, act, s_act, group=8 if (n // 2) % 8 == 0 else 0)}
+    for fn in (steps["norm"], steps["product"], steps["gated"]):
+        fn(0)
+    us = {name: _time_graph(fn, reps) for name, fn in steps.items()}
+    print(f"float8 M={m} N={n} K={k}: product {us['product']:8.2f} us  {n * k / us['product'] / 1e3:7.0f} GB/s of weights  {2 * m * n * k / us['product'] / 1e6:7.0f} TFLOP/s"
+          f"  norm {us['norm']:7.2f} us  gated {us['gated']:7.2f} us", flush=True)
 
 
 def gemm_case(m: int, n: int, k: int, epilogue: int, reps: int = 10, splits: int = 1) -> None:
@@ -199,6 +223,8 @@ def main(argv=None) -> int:
     p.add_argument("--m", type=int, default=2048); p.add_argument("--n", type=int, default=24576)
     p.add_argument("--k", type=int, default=4096); p.add_argument("--epilogue", type=int, default=0)
     p.add_argument("--splits", type=int, default=1, help="ranges of K into float32 partial products; -1: what the engine would ask for")
+    p = sub.add_parser("float8")
+    p.add_argument("--m", type=int, default=8); p.add_argument("--n", type=int, default=24576); p.add_argument("--k", type=int, default=4096)
     p = sub.add_parser("attn-decode")
     p.add_argument("--batch", type=int, default=1); p.add_argument("--ctx", type=int, default=1030)
     p.add_argument("--impl", default="stream", choices=["stream", "direct"]); p.add_argument("--page", type=int, default=16)
@@ -220,6 +246,8 @@ def main(argv=None) -> int:
         gemv_case(args.n, args.k, args.m, args.epilogue)
     elif args.case == "gemm":
         gemm_case(args.m, args.n, args.k, args.epilogue, splits=args.splits)
+    elif args.case == "float8":
+        float8_case(args.m, args.n // 2 * 2, args.k)
     elif args.case == "attn-decode":
         attn_decode_case(args.batch, args.ctx, page=args.page, impl=args.impl)
     elif args.case == "attn-prefill":
@@ -237,6 +265,10 @@ def main(argv=None) -> int:
             for name, (n, k, epi) in shapes.items():
                 if name != "head":
                     gemm_case(m, n, k, epi)
+        for m in (1, 8, 64, 2048):
+            for name, (n, k, _) in shapes.items():
+                if name != "head":
+                    float8_case(m, n, k)
         for impl in ("stream", "direct"):
             for b in (1, 8, 64):
                 attn_decode_case(b, 1030, impl=impl)

@@ -895,6 +895,8 @@ def main() -> int:
         print(f"bench.py measures a single-GPU engine: --gpus {args.gpus} is not supported (use --gpus 1)")
         return 2
     warmup, steps = max(3, args.warmup), max(1, args.steps)
+    if args.weights != "stored" and args.workload not in WORKLOADS:
+        ap.error(f"--weights {args.weights} belongs to the workloads {', '.join(WORKLOADS)}")
     if args.workload == "serving":
         return serving_workload(args.align_step_tokens)
     if args.workload == "mixed_step":
