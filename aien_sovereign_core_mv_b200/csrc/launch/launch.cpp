@@ -7,6 +7,7 @@
 //   matrix(t, rows, cols, types)     numbers between the rows of t (of a single row: its length) where t is a matrix of this size on the current
 //                                    CUDA device, of a type in types (1 float32, 2 bfloat16, 4 e4m3 added up; 8: contiguous), its rows whole and apart; -1 otherwise;
 //                                    with 16 added to types, how many such matrices t [parts, rows, cols] holds
+//   sizes(t)                         (rows, columns) of a matrix, (-1, -1) of anything else
 //
 // Through ctypes a call of 29 arguments takes 4.2 us (and 0.25 us more a tensor for its address), here 0.5 us; as_strided 2.3 us
 // and strided 0.5 us.  A layer's step makes six to eleven calls and as many views.
@@ -199,6 +200,16 @@ PyObject* matrix(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
 }
 
+PyObject* sizes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 1 || !THPVariable_Check(args[0])) {
+        PyErr_SetString(PyExc_TypeError, "sizes(tensor)");
+        return nullptr;
+    }
+    const at::Tensor& t = THPVariable_Unpack(args[0]);
+    const bool two = t.dim() == 2;
+    return Py_BuildValue("LL", two ? (long long)t.size(0) : -1LL, two ? (long long)t.size(1) : -1LL);
+}
+
 template <typename F>
 PyCFunction fast(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)); }
 
@@ -207,6 +218,7 @@ PyMethodDef methods[] = {
     {"on_device", fast(on_device), METH_FASTCALL, nullptr},
     {"strided", fast(strided), METH_FASTCALL, nullptr},
     {"matrix", fast(matrix), METH_FASTCALL, nullptr},
+    {"sizes", fast(sizes), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -175,13 +175,16 @@ class stream_scope:
         return False
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # the current stream's handle without an object around it: 0.2 us for 1.0
+# the current stream's handle without an object around it: 0.2 us for 3.2
+_raw_stream, _device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _stream() -> int:
     if _STREAM is not None:
         return _STREAM
-    return _raw_stream(torch.cuda.current_device()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None or _device is None or not torch.cuda.is_initialized():
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_device())
 
 
 def dt(t: torch.Tensor) -> int:
@@ -2488,12 +2491,10 @@ def _rows_of(name: str, what: str, t: torch.Tensor, shape: tuple, dtypes: tuple)
 
 def _two(name: str, t: torch.Tensor) -> tuple:
     """(rows, columns) of a matrix with columns."""
-    if t.dim() != 2:
-        _refuse(name, f"a matrix is wanted, not {t.dim()} dimensions")
-    rows, cols = t.shape
-    if cols < 1:
-        _refuse(name, "rows of no numbers")
-    return rows, cols
+    got = _sizes(t)
+    if got[1] < 1:
+        _refuse(name, "rows of no numbers" if got[1] == 0 else f"a matrix is wanted, not {t.dim()} dimensions")
+    return got
 
 
 def _whole(name: str, what: str, t: torch.Tensor) -> torch.Tensor:
@@ -2525,6 +2526,13 @@ def _matrix(t: torch.Tensor, rows: int, cols: int, types: int) -> int:
     return _matrix(t, rows, cols, types)
 
 
+def _sizes(t: torch.Tensor) -> tuple:
+    """(rows, columns) of a matrix, (-1, -1) of anything else (the native function takes this one's place)."""
+    global _sizes
+    _sizes = _build.load_launch().sizes
+    return _sizes(t)
+
+
 def _explain(name: str, *wanted) -> None:
     """Raises what is wrong with the first of (what, tensor, shape, dtypes) that is not as wanted, or with where one of them lives."""
     for what, t, shape, dtypes in wanted:
@@ -2537,7 +2545,7 @@ def quantize_rows_float8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Ten
     """x [T, K] float32 or bfloat16 (row stride free) in 8 bits: codes [T, K] e4m3, scales [ceil(K / 128), T] float32."""
     name = "quantize_rows_float8"
     T, width = _two(name, codes)
-    blocks = float8_blocks(width)
+    blocks = (width + 127) // 128
     ldx, ldc, lds = _matrix(x, T, width, 3), _matrix(codes, T, width, 4), _matrix(scales, blocks, T, 1)
     if ldx < 0 or ldc < 0 or lds < 0:
         _explain(name, ("x", x, (T, width), _F32_BF16), ("codes", codes, (T, width), _E4M3), ("scales", scales, (blocks, T), _F32))
@@ -2549,7 +2557,7 @@ def swiglu_float8(gate_up: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     as codes [T, K] and scales [ceil(K / 128), T]."""
     name = "swiglu_float8"
     T, width = _two(name, codes)
-    blocks = float8_blocks(width)
+    blocks = (width + 127) // 128
     if act not in GATED_ACTS:
         _refuse(name, f"activation {act!r}: known are {sorted(GATED_ACTS)}")
     if group < 0 or (group > 0 and width % group):
@@ -2566,7 +2574,7 @@ def add_rmsnorm_float8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: t
     products [P, T, H]) in place; rmsnorm(x) * weight as codes [T, H] and scales [ceil(H / 128), T]."""
     name = "add_rmsnorm_float8"
     T, H = _two(name, codes)
-    blocks = float8_blocks(H)
+    blocks = (H + 127) // 128
     ldx, ldc, lds = _matrix(x, T, H, 1 + 8), _matrix(codes, T, H, 4), _matrix(scales, blocks, T, 1)
     nparts, stride = 1, 0
     if delta is not None:
@@ -2610,10 +2618,10 @@ def matmul_float8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_sc
     it may be requested ahead of their end."""
     name = "matmul_float8"
     width = _two(name, a)[1]
-    if out.dim() != 2:
+    M, N = _sizes(out)
+    if M < 0:
         _refuse(name, f"a matrix is wanted, not {out.dim()} dimensions")
-    M, N = out.shape
-    blocks, n_blocks = float8_blocks(width), float8_blocks(N)
+    blocks, n_blocks = (width + 127) // 128, (N + 127) // 128
     lda, ldsa, ldw = _matrix(a, M, width, 4), _matrix(a_scales, blocks, M, 1), _matrix(w, N, width, 4)
     ldsw, ldo = _matrix(w_scales, n_blocks, blocks, 1), _matrix(out, M, N, 3)
     if lda < 0 or ldsa < 0 or ldw < 0 or ldsw < 0 or ldo < 0:
