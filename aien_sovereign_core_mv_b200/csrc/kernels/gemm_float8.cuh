@@ -235,6 +235,7 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
             mbar_wait(tfull0 + 8 * t.at, t.parity, 3);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            __syncwarp();                                                     // (the loads of tensor memory are the whole warp's)
             const ulonglong2* f = reinterpret_cast<const ulonglong2*>(factors + (kb % C::CHUNK) * NT);
 #pragma unroll
             for (int c0 = 0; c0 < NT; c0 += 16) {
@@ -285,6 +286,7 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
         __syncwarp();
         if (warp >= 2) f8_wait_cluster(parts_in, 0, 3);
+        __syncwarp();
         asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); // what others sent has arrived: when everyone says so, everyone may leave
         if (warp >= 2) {
             // Added up in the order of K.  Where two numbers make an aligned word, a thread takes two neighbours of every other column (one number of
@@ -761,6 +763,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 }
                 mbar_wait(tfull0 + 8 * t.at, t.parity, 3);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                __syncwarp();                                                 // (the loads of tensor memory are the whole warp's)
                 f8_add_block<W>(columns + t.at * C::BN, f.x, acc, [&]() {
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
