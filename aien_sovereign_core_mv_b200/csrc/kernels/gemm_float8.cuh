@@ -383,7 +383,7 @@ __device__ __forceinline__ void f8_add_block(uint32_t taddr, float f, float (&ac
     }
 }
 
-// A warp's 32 rows x W columns of the result, a row a lane.  By TMA (the result's rows start on 16-byte borders): 128 bytes of a row at a time into
+// A warp's 32 rows x W columns of the result, a row a lane.  By TMA (the result's rows start and end on 16-byte borders): 128 bytes of a row at a time into
 // a buffer of 4 KB, 16-byte pieces swizzled as the copy expects them; rows and columns beyond the matrix are clipped by it.
 // Other results leave the buffer row after row.  Stored from registers each lane's 16 bytes are a row of their own (a tile of 128 x 256 took 6,700 cycles so).
 constexpr int F8_STORE = 4096;
@@ -860,7 +860,8 @@ int launch_float8_tiles(const void* a, long lda, const void* w, long ldw, F8Scal
     constexpr int P = C::P;
     CUtensorMap ma = {}, mw = {}, mo = {};
     if (!GATHER && (!f8_make_map(&ma, a, M, K, lda, 128) || !f8_make_map(&mw, w, N, K, ldw, 128))) return AIEN_E_STATE;
-    const bool by_tma = !GATED && ((uintptr_t)out & 15) == 0 && (M == 1 || ldc * sizeof(TC) % 16 == 0);
+    // (a copy out writes whole 16-byte words: a row that ends inside one would take what lies behind it along)
+    const bool by_tma = !GATED && ((uintptr_t)out & 15) == 0 && (M == 1 || ldc * sizeof(TC) % 16 == 0) && (long)N * sizeof(TC) % 16 == 0;
     if (by_tma && !f8_make_map_out<TC>(&mo, out, M, N, ldc)) return AIEN_E_STATE;
     constexpr auto kernel = float8_tiles_kernel<PAIR, GATHER, GATED, TC>;
     if (!f8_configure<kernel, C::SMEM>()) return AIEN_E_STATE;

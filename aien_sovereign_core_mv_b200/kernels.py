@@ -2593,6 +2593,7 @@ def add_rmsnorm_float8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: t
             wanted.append(("delta", _whole(name, "delta", delta).view(P * T, H), (P * T, H), _F32))
         elif delta is not None:
             wanted.append(("delta", _whole(name, "delta", delta), (T, H), _F32_BF16))
+        _here(name, weight)
         _explain(name, *wanted)
     _check(lib().aien_add_rmsnorm_float8(x, delta, F32 if delta is None else dt(delta), nparts, stride, weight, dt(weight), float(eps),
                                          codes, ldc, scales, lds, T, H, _stream()), name)

@@ -230,6 +230,22 @@ def test_product_of_rows_apart(K, out_dtype, M, N, width, gap_a, gap_w, gap_out)
     assert bool((whole[:, N:] == 5.0).all())
 
 
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("width", [48, 55, 400])
+@pytest.mark.parametrize("N", [1, 3, 7, 130, 257, 735, 1034])
+@pytest.mark.parametrize("M", [1, 5, 40, 130, 400, 900])
+def test_nothing_is_written_beyond_the_result(K, M, N, width, out_dtype):
+    """Rows of the result that start on 16-byte borders and end inside a word, with others' numbers behind them."""
+    a, w = codes_of(M, M, width), codes_of(N, N, width)
+    b = K.float8_blocks(width)
+    sa, sw = scales_of(3, b, M), scales_of(4, K.float8_blocks(N), b)
+    for ld in ((N + 8) // 8 * 8, N + 1, N + 9):
+        whole = torch.full((M + 2, ld), 5.0, dtype=out_dtype, device="cuda")
+        K.matmul_float8(a, sa, w, sw, whole[1:M + 1, :N])
+        check_product(whole[1:M + 1, :N], a, sa, w, sw)
+        assert bool((whole[:, N:] == 5.0).all()) and bool((whole[0] == 5.0).all()) and bool((whole[M + 1] == 5.0).all())
+
+
 @pytest.mark.parametrize("M", [4, 40, 200, 600])
 def test_product_starts_anywhere(K, M):
     """Rows that begin off the 16-byte borders: a view of a larger tensor."""
@@ -241,11 +257,11 @@ def test_product_starts_anywhere(K, M):
     check_product(out, a, sa, w, sw)
 
 
-@pytest.mark.parametrize("at,gap", [(0, 16), (16, 32), (1, 3), (15, 0), (5, 11)])
+@pytest.mark.parametrize("at,gap", [(0, 16), (16, 32), (1, 3), (15, 0), (5, 11), (0, "border"), (32, "border")])
 @pytest.mark.parametrize("M,N,width", [(1, 130, 120), (20, 130, 129), (100, 200, 1000), (300, 260, 257), (600, 1030, 400)])
 def test_what_lies_around_the_rows_is_not_looked_at(K, M, N, width, at, gap):
     """Codes that are not numbers before, between and behind the rows; scales that are not numbers beside the ones that count."""
-    ld = width + at + gap
+    ld = width + at + gap if gap != "border" else (width + at + 16) // 16 * 16         # rows that start on 16-byte borders and end inside one
     def among_nan(seed, rows):
         whole = torch.full((rows + 2, ld), 0x7f, dtype=torch.uint8, device="cuda").view(E4M3)
         part = whole[1:rows + 1, at:at + width]
@@ -340,6 +356,16 @@ def test_gated_product_refusals(K):
         K.matmul_swiglu_float8(a, sa, codes_of(3, 40, 256), scales_of(4, 1, 2), *out(24))
     with pytest.raises(K.KernelError, match="aligned"):
         K.matmul_swiglu_float8(codes_of(1, 5, 250), sa, codes_of(3, 48, 250), scales_of(4, 1, 2), *out(24))
+
+
+def test_arguments_on_the_host_are_refused(K):
+    x, codes, scales, w = randn(1, 3, 256), codes_of(2, 3, 256), scales_of(3, 2, 3), torch.ones(256, device="cuda")
+    for bad in (dict(weight=w.cpu()), dict(x=x.cpu()), dict(scales=scales.cpu()), dict(delta=x.cpu())):
+        args = {**dict(x=x, delta=None, weight=w, eps=1e-6, codes=codes, scales=scales), **bad}
+        with pytest.raises(K.KernelError, match="CUDA device"):
+            K.add_rmsnorm_float8(**args)
+    with pytest.raises(K.KernelError, match="CUDA device"):
+        K.quantize_rows_float8(x, codes.cpu(), scales)
 
 
 def test_nothing_to_do(K):
