@@ -941,7 +941,8 @@ static int tc_num_sms() {
 // Whether a product's float32 results can leave by TMA (see tc_store_tma), and the map for them.
 template <int EPI, typename TC>
 static int tc_store_map(CUtensorMap* map, const void* out, long ldc, int M, int N, int parts, size_t part_stride) {
-    if (sizeof(TC) != 4 || EPI != 0 || (ldc & 3) || (part_stride & 3) || ((uintptr_t)out & 15)) return 0;
+    // (the copy writes whole 16-byte words: a row that ends inside one would take what lies behind it along)
+    if (sizeof(TC) != 4 || EPI != 0 || (ldc & 3) || (N & 3) || (part_stride & 3) || ((uintptr_t)out & 15)) return 0;
     return make_map_store_f32(map, out, (uint64_t)M, (uint64_t)N, (uint64_t)ldc, (uint64_t)parts, (uint64_t)part_stride) ? 1 : 0;
 }
 
