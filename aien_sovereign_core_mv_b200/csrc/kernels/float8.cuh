@@ -19,13 +19,76 @@ __device__ __forceinline__ float f8_reciprocal(float v) {
     return r;
 }
 __device__ __forceinline__ float f8_inverse(float scale) { return f8_reciprocal(scale); }
-// act(g) * u: silu, or the gelu in its tanh form, from one exponential and one reciprocal (for large -g the exponential is infinite, its reciprocal 0).
-template <bool GELU>
-__device__ __forceinline__ float f8_gate(float g, float u) {
-    if (GELU) return 0.5f * g * (1.0f + tanh_ex2(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
+
+// ---------------------------------------------------------------- gated activations
+// One float32 number, or two in a pair of registers that one instruction takes.
+__device__ __forceinline__ uint64_t f8_two(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
+    return v;
+}
+__device__ __forceinline__ float2 f8_split(uint64_t v) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ float f8_ex2(float v) {
     float t;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -1.4426950408889634f));
-    return g * f8_reciprocal(1.0f + t) * u;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(v));
+    return t;
+}
+template <typename V> struct F8Math;
+template <> struct F8Math<float> {
+    using V = float;
+    static __device__ __forceinline__ V all(float v) { return v; }
+    static __device__ __forceinline__ V mul(V a, V b) { return __fmul_rn(a, b); }                        // (never one instruction with an addition)
+    static __device__ __forceinline__ V add(V a, V b) { return __fadd_rn(a, b); }
+    static __device__ __forceinline__ V mad(V a, V b, V c) { return fmaf(a, b, c); }
+    static __device__ __forceinline__ V larger(V a, V b) { return fmaxf(a, b); }
+    static __device__ __forceinline__ V minus_abs(V a, float least) { return fmaxf(-fabsf(a), least); }
+    static __device__ __forceinline__ V ex2(V a) { return f8_ex2(a); }
+    static __device__ __forceinline__ V minus_reciprocal(V a) { return f8_reciprocal(-a); }
+};
+template <> struct F8Math<uint64_t> {
+    using V = uint64_t;
+    static __device__ __forceinline__ V all(float v) { return f8_two(v, v); }
+    static __device__ __forceinline__ V mul(V a, V b) { V r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+    static __device__ __forceinline__ V add(V a, V b) { V r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+    static __device__ __forceinline__ V mad(V a, V b, V c) { V r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+    template <typename F> static __device__ __forceinline__ V each(V a, F f) { const float2 x = f8_split(a); return f8_two(f(x.x), f(x.y)); }
+    static __device__ __forceinline__ V larger(V a, V b) { const float2 x = f8_split(a), y = f8_split(b); return f8_two(fmaxf(x.x, y.x), fmaxf(x.y, y.y)); }
+    static __device__ __forceinline__ V minus_abs(V a, float least) { return each(a, [=](float v) { return fmaxf(-fabsf(v), least); }); }
+    static __device__ __forceinline__ V ex2(V a) { return each(a, [](float v) { return f8_ex2(v); }); }
+    static __device__ __forceinline__ V minus_reciprocal(V a) { return each(a, [](float v) { return f8_reciprocal(-v); }); }
+};
+// -g / (1 + exp(-x)), x of g's sign: -max(g, g e) / (1 + e) with e = exp(-|x|), so that the divisor lies between 1 and 2 and a small result is as exact as
+// a large one.  e is 2^p times a correction by what p = -|x| log2(e), rounded, lacks (rest: |x| 2^-24 at the most, which the instruction
+// alone would be off by, relatively); it is made 2^24 times as large, so that the instruction's flush of small numbers to 0 stays below |x| = 103, where e leaves
+// float32.  Adding 24 to p rounds it again; taking 24 off the sum again is exact.  The quotient is a product with an approximate reciprocal, corrected
+// by its exact residue (Markstein, 1990): next to always the rounded quotient.  In all 9 half steps of float32 at the most, beside what x is off.
+// (The sign is the reciprocal's, whose operand may be negated; the residue is then one product with the divisor as it is.)
+template <typename V>
+__device__ __forceinline__ V f8_minus_logistic(V g, V x) {
+    using F = F8Math<V>;
+    const V a = F::minus_abs(x, -200.0f), up = F::add(F::mul(a, F::all(1.44269504f)), F::all(24.0f)), p = F::add(up, F::all(-24.0f));
+    const V rest = F::mad(p, F::all(1.90465430e-9f), F::mad(p, F::all(-0.693147182f), a));              // a - p ln 2, ln 2 in two parts
+    const V t = F::ex2(up), e = F::mad(t, rest, t), d = F::mad(e, F::all(0x1p-24f), F::all(1.0f));
+    const V n = F::larger(g, F::mul(F::mul(g, e), F::all(0x1p-24f))), r = F::minus_reciprocal(d), q = F::mul(n, r);
+    return F::mad(F::mad(q, d, n), r, q);
+}
+// -act(g) * u: silu, or the gelu in its tanh form.
+template <bool GELU>
+__device__ __forceinline__ float f8_minus_gate(float g, float u) {
+    if (GELU) return -0.5f * g * (1.0f + tanh_ex2(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
+    return f8_minus_logistic<float>(g, g) * u;
+}
+template <bool GELU>
+__device__ __forceinline__ uint64_t f8_minus_gate(uint64_t g, uint64_t u) {
+    if (GELU) {
+        const float2 a = f8_split(g), b = f8_split(u);
+        return f8_two(f8_minus_gate<GELU>(a.x, b.x), f8_minus_gate<GELU>(a.y, b.y));
+    }
+    return F8Math<uint64_t>::mul(f8_minus_logistic<uint64_t>(g, g), u);
 }
 __device__ __forceinline__ uint32_t f8_pair(float a, float b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);

@@ -60,16 +60,6 @@ __device__ __forceinline__ void f8_fma2(uint64_t& acc, uint32_t v0, uint32_t v1,
     asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(v0), "r"(v1));
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
 }
-__device__ __forceinline__ uint64_t f8_two(float a, float b) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
-    return v;
-}
-__device__ __forceinline__ float2 f8_split(uint64_t v) {
-    uint32_t a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-    return make_float2(__uint_as_float(a), __uint_as_float(b));
-}
 __device__ __forceinline__ void f8_named_barrier(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 
 __device__ __forceinline__ float4 f8_lds4(uint32_t at) {
@@ -547,18 +537,24 @@ struct F8Gated8 {
     long lds;
     int gelu;
 };
-// act(gate) * up of a row's 128 columns, which hold gate and up in runs of 8, in 8 bits.  A tile's 256 columns give the 128 numbers of one block: the two
-// threads of a row tell each other their largest (`tops`, two floats a row).  All of it is float32: the columns are never rounded to 16 bits.
-__device__ __forceinline__ void f8_store_gated(float (&acc)[128], const F8Gated8& g, uint32_t tops, int half, int row, int m, int n, int M, int N) {
+// act(gate) * up of 128 columns in runs of 8, in the first 64 of them; their largest
+template <bool GELU>
+__device__ __forceinline__ uint32_t f8_gate_columns(float (&acc)[128], int n, int N) {
     uint32_t top = 0;
 #pragma unroll
     for (int v = 0; v < 8; ++v)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float y = g.gelu ? f8_gate<true>(acc[16 * v + j], acc[16 * v + 8 + j]) : f8_gate<false>(acc[16 * v + j], acc[16 * v + 8 + j]);
+            const float y = -f8_minus_gate<GELU>(acc[16 * v + j], acc[16 * v + 8 + j]);
             acc[8 * v + j] = y;
             if (n + 16 * v < N) top = max(top, f8_bits(y));
         }
+    return top;
+}
+// act(gate) * up of a row's 128 columns, which hold gate and up in runs of 8, in 8 bits.  A tile's 256 columns give the 128 numbers of one block: the two
+// threads of a row tell each other their largest (`tops`, two floats a row).  All of it is float32: the columns are never rounded to 16 bits.
+__device__ __forceinline__ void f8_store_gated(float (&acc)[128], const F8Gated8& g, uint32_t tops, int half, int row, int m, int n, int M, int N) {
+    const uint32_t top = g.gelu ? f8_gate_columns<true>(acc, n, N) : f8_gate_columns<false>(acc, n, N);
     asm volatile("st.shared.b32 [%0], %1;" ::"r"(tops + (half * 128 + row) * 4), "r"(top) : "memory");
     asm volatile("bar.sync 2, 256;" ::: "memory");
     uint32_t other;
