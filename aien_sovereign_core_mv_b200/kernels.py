@@ -2533,11 +2533,11 @@ def _sizes(t: torch.Tensor) -> tuple:
     return _sizes(t)
 
 
-def _explain(name: str, *wanted) -> None:
-    """Raises what is wrong with the first of (what, tensor, shape, dtypes) that is not as wanted, or with where one of them lives."""
+def _explain(name: str, *wanted, also: tuple = ()) -> None:
+    """Raises what is wrong with the first of (what, tensor, shape, dtypes) that is not as wanted, or with where one of them or of ``also`` lives."""
     for what, t, shape, dtypes in wanted:
         _rows_of(name, what, t, shape, dtypes)
-    _here(name, *(t for _, t, _, _ in wanted))
+    _here(name, *(t for _, t, _, _ in wanted), *also)
     _refuse(name, "an argument is not what it should be")
 
 
@@ -2593,8 +2593,7 @@ def add_rmsnorm_float8(x: torch.Tensor, delta: Optional[torch.Tensor], weight: t
             wanted.append(("delta", _whole(name, "delta", delta).view(P * T, H), (P * T, H), _F32))
         elif delta is not None:
             wanted.append(("delta", _whole(name, "delta", delta), (T, H), _F32_BF16))
-        _here(name, weight)
-        _explain(name, *wanted)
+        _explain(name, *wanted, also=(weight,))
     _check(lib().aien_add_rmsnorm_float8(x, delta, F32 if delta is None else dt(delta), nparts, stride, weight, dt(weight), float(eps),
                                          codes, ldc, scales, lds, T, H, _stream()), name)
 
