@@ -76,19 +76,14 @@ __device__ __forceinline__ V f8_minus_logistic(V g, V x) {
     const V n = F::larger(g, F::mul(F::mul(g, e), F::all(0x1p-24f))), r = F::minus_reciprocal(d), q = F::mul(n, r);
     return F::mad(F::mad(q, d, n), r, q);
 }
-// -act(g) * u: silu, or the gelu in its tanh form.
-template <bool GELU>
-__device__ __forceinline__ float f8_minus_gate(float g, float u) {
-    if (GELU) return -0.5f * g * (1.0f + tanh_ex2(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
-    return f8_minus_logistic<float>(g, g) * u;
-}
-template <bool GELU>
-__device__ __forceinline__ uint64_t f8_minus_gate(uint64_t g, uint64_t u) {
-    if (GELU) {
-        const float2 a = f8_split(g), b = f8_split(u);
-        return f8_two(f8_minus_gate<GELU>(a.x, b.x), f8_minus_gate<GELU>(a.y, b.y));
-    }
-    return F8Math<uint64_t>::mul(f8_minus_logistic<uint64_t>(g, g), u);
+// -act(g) * u: silu, or the gelu in its tanh form, 0.5 g (1 + tanh z) = g / (1 + exp(-2 z)) with z = sqrt(2 / pi) (g + 0.044715 g^3).  (As 1 + tanh z nothing
+// would be left of it for gates below -5.)
+template <bool GELU, typename V>
+__device__ __forceinline__ V f8_minus_gate(V g, V u) {
+    using F = F8Math<V>;
+    V x = g;
+    if (GELU) x = F::mul(g, F::mad(F::mul(g, g), F::all(0.0713548163f), F::all(1.59576912f)));           // 2 z
+    return F::mul(f8_minus_logistic<V>(g, x), u);
 }
 __device__ __forceinline__ uint32_t f8_pair(float a, float b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);

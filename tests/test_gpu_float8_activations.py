@@ -48,7 +48,7 @@ def check(scales, want, units):
     assert bool((far <= 0).all()), f"{float(far.max())} units beyond"
 
 
-@pytest.mark.parametrize("act", ["silu"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
 def test_one_number_a_row(K, act):
     """Every gate in a row of its own, times 2^24, so that no scale is the least one."""
     g = gates(act)
@@ -59,7 +59,7 @@ def test_one_number_a_row(K, act):
     check(scales[0], f * 2.0 ** 24, units)
 
 
-@pytest.mark.parametrize("act", ["silu"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
 def test_one_number_a_row_of_a_gated_product(K, act):
     """gate = the row's scale times its sign, up = 256 times that: one k whose codes are 1 and 256, eight columns that are the same."""
     g = gates(act)
@@ -76,7 +76,7 @@ def test_one_number_a_row_of_a_gated_product(K, act):
     assert K.read_wait_errors() == (0, 0, 0, 0)
 
 
-@pytest.mark.parametrize("act", ["silu"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
 @pytest.mark.parametrize("width", [1, 8])
 def test_gates_of_any_size(K, act, width):
     """Up to the largest float32 number the activation is the gate, or 0; one that is not finite leaves a block that is none."""
@@ -91,7 +91,7 @@ def test_gates_of_any_size(K, act, width):
     assert bool(torch.isnan(codes[2 * n:].float()).all()) and bool(torch.isnan(scales[0, 2 * n:]).all())
 
 
-@pytest.mark.parametrize("act", ["silu"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
 @pytest.mark.parametrize("group", [0, 8])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_blocks_of_small_activations(K, act, group, dtype):
