@@ -12,13 +12,19 @@ __device__ __forceinline__ uint32_t f8_bits(float v) { return __float_as_uint(fa
 __device__ __forceinline__ float f8_scale(uint32_t top) {
     return top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(top) * (1.0f / F8_TOP), F8_LEAST);
 }
-// One instruction of the special-function unit, at most a unit off; a scale and its reciprocal are ordinary numbers (2^-126 to 2^120).
+// One instruction of the special-function unit, at most a unit off, for ordinary numbers.
 __device__ __forceinline__ float f8_reciprocal(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ float f8_inverse(float scale) { return f8_reciprocal(scale); }
+// 1 / scale as float32 rounds it, so that a code is e4m3(x * (1 / scale)) to the bit: the instruction's result, corrected once by its exact residue (Markstein, 1990;
+// compared with the rounded quotient over all mantissas at eight exponents).  A scale and its reciprocal are ordinary numbers, 2^-126 to 2^120.  Gated
+// rows of 2,048 x 12,288 in 25.0 us, with a division 26.0.
+__device__ __forceinline__ float f8_inverse(float scale) {
+    const float r = f8_reciprocal(scale);
+    return fmaf(fmaf(-scale, r, 1.0f), r, r);
+}
 
 // ---------------------------------------------------------------- gated activations
 // One float32 number, or two in a pair of registers that one instruction takes.
