@@ -106,6 +106,21 @@ __device__ __forceinline__ void f8_wait_cluster(uint32_t bar, uint32_t parity, i
     atomicCAS(&g_wait_error, 0, code);
 }
 
+// All loads of tensor memory so far are in r.  (r goes through the wait: what is made of it in registers alone, which no order of volatile statements holds
+// back, cannot be moved ahead of it.)
+__device__ __forceinline__ void f8_tmem_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+}
+__device__ __forceinline__ void f8_tmem_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+    asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                   "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+
 // bytes of this CTA's shared memory to another one's of the cluster, which counts at a barrier there
 __device__ __forceinline__ void f8_copy_to_rank(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
@@ -231,7 +246,7 @@ float8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             for (int c0 = 0; c0 < NT; c0 += 16) {
                 uint32_t r[16];
                 tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(t.at * NT + c0), r);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                f8_tmem_wait(r);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const ulonglong2 s2 = f[c0 / 4 + j];
@@ -343,14 +358,6 @@ __device__ __forceinline__ void f8_copy_scales(uint32_t dst, uint32_t bar, const
         f8_copy4(dst + (128 * F8_BATCH + lane) * 4, live ? sc.w + (long)n * sc.ldw + k : sc.w, live);
     }
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-// all loads of tensor memory so far are in r
-__device__ __forceinline__ void f8_tmem_wait(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
-    asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
-                   "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
 // acc += (W columns of a k-block's sums at taddr) * f; the next 32 columns are on their way while 32 are added.  read(): called when the last of
 // them has left tensor memory.
