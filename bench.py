@@ -12,7 +12,8 @@ line is printed:
 * ``e2e``        the same through the Python entry point (scheduler, sampling, token ids from and
                  to the host every step);
 * ``prefill``    one 2,048-token prompt in one step: tokens per second and the fraction of the
-                 bfloat16 tensor peak its flops reach;
+                 bfloat16 tensor peak its flops reach (with ``--weights float8`` the layers' products
+                 are set against twice that peak);
 * ``roofline``   bytes a decode step must read (every weight once, the cache of the live
                  requests) per second against the measured copy bandwidth;
 * ``points``     decode tokens per second at batch 1 and 64.
@@ -134,6 +135,14 @@ def model_numbers(cfg, layers_run, weights="stored"):
     layer_bytes = per_layer * layers_run * (1 + 4 / 128 ** 2) if weights == "float8" else 2 * per_layer * layers_run
     return dict(per_layer=per_layer, linear_params=linear_params, weight_bytes=int(layer_bytes + 2 * (V * H + norm_params)),
                 kv_bytes_per_token=kv_bytes_per_token, Q=Q, KV=KV)
+
+
+def prefill_floor_s(cfg, nums, layers_run, tokens, bf16_tflops, weights="stored"):
+    """Seconds that one prompt takes at the tensor cores' peak: the layers' products at the rate of their type (8 bits: twice the
+    measured bfloat16 rate), attention and the one row of logits at the bfloat16 rate."""
+    products = 2.0 * nums["per_layer"] * layers_run * tokens
+    others = 2.0 * cfg["vocab_size"] * cfg["hidden_size"] + layers_run * 4.0 * nums["Q"] * tokens * (tokens + 1) / 2
+    return (products / (2.0 if weights == "float8" else 1.0) + others) / (bf16_tflops * 1e12)
 
 
 QWEN3_4B = dict(
@@ -1044,10 +1053,10 @@ def main() -> int:
         count_wait_errors()
         pms = float(np.median(times[3:]))
         T = ptok
-        flops = 2.0 * (nums["linear_params"] - V * cfg["hidden_size"]) * T + 2.0 * V * cfg["hidden_size"] \
-            + layers_run * 4.0 * nums["Q"] * T * (T + 1) / 2
+        floor_s = prefill_floor_s(cfg, nums, layers_run, T, bf16_tflops, args.weights)
+        peak = f"{bf16_tflops} TFLOP/s bf16" + (", twice that for the layers' products" if args.weights == "float8" else "")
         return {"value": round(T / (pms / 1e3), 1), "tokens": T, "ms": round(pms, 3), "runs_ms": [round(t, 2) for t in times],
-                "frac": round(flops / (pms / 1e3) / (bf16_tflops * 1e12), 4), "peak": f"{bf16_tflops} TFLOP/s bf16, of {peak_src}"}
+                "frac": round(floor_s / (pms / 1e3), 4), "peak": f"{peak}, of {peak_src}"}
 
     # the prefill is timed before the decode runs, as a burst, like the peak it is set against
     prefill = None if args.skip_prefill else prefill_run()
