@@ -380,7 +380,7 @@ __device__ __forceinline__ void f8_add_block(uint32_t taddr, float f, float (&ac
     }
 }
 
-// A warp's 32 rows x W columns of the result, a row a lane.  By TMA (the result's rows start and end on 16-byte borders): 128 bytes of a row at a time into
+// A warp's 32 rows x W columns of the result, a row a lane.  By TMA (the result's rows start on 16-byte borders): 128 bytes of a row at a time into
 // a buffer of 4 KB, 16-byte pieces swizzled as the copy expects them; rows and columns beyond the matrix are clipped by it.
 // Other results leave the buffer row after row.  Stored from registers each lane's 16 bytes are a row of their own (a tile of 128 x 256 took 6,700 cycles so).
 constexpr int F8_STORE = 4096;
@@ -390,6 +390,8 @@ __device__ __forceinline__ void f8_store_rows(const float (&acc)[W], const CUten
     constexpr int COLS = 128 / sizeof(TC);
 #pragma unroll
     for (int c0 = 0; c0 < W; c0 += COLS) {
+        // (a copy writes whole 16-byte words: a box in which rows end inside one would take what lies behind them along)
+        const bool leaves = by_tma && (n + c0 + COLS <= N || N % (16 / (int)sizeof(TC)) == 0);
         if (by_tma && lane == 0) tma_store_read<0>();                         // the last copy has read the buffer
         __syncwarp();
 #pragma unroll
@@ -408,7 +410,7 @@ __device__ __forceinline__ void f8_store_rows(const float (&acc)[W], const CUten
             }
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 128 + ((p ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
         }
-        if (by_tma) {
+        if (leaves) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
@@ -417,7 +419,7 @@ __device__ __forceinline__ void f8_store_rows(const float (&acc)[W], const CUten
             }
         } else {                                                              // row after row, neighbouring lanes neighbouring numbers
             __syncwarp();
-            const int end = min(32, M - m);
+            const int end = n + c0 < N ? min(32, M - m) : 0;
 #pragma unroll 4
             for (int r = 0; r < end; ++r) {
                 TC* to = out + (long)(m + r) * ldc + n + c0;
@@ -863,8 +865,7 @@ int launch_float8_tiles(const void* a, long lda, const void* w, long ldw, F8Scal
     constexpr int P = C::P;
     CUtensorMap ma = {}, mw = {}, mo = {};
     if (!GATHER && (!f8_make_map(&ma, a, M, K, lda, 128) || !f8_make_map(&mw, w, N, K, ldw, 128))) return AIEN_E_STATE;
-    // (a copy out writes whole 16-byte words: a row that ends inside one would take what lies behind it along)
-    const bool by_tma = !GATED && ((uintptr_t)out & 15) == 0 && (M == 1 || ldc * sizeof(TC) % 16 == 0) && (long)N * sizeof(TC) % 16 == 0;
+    const bool by_tma = !GATED && ((uintptr_t)out & 15) == 0 && (M == 1 || ldc * sizeof(TC) % 16 == 0);
     if (by_tma && !f8_make_map_out<TC>(&mo, out, M, N, ldc)) return AIEN_E_STATE;
     constexpr auto kernel = float8_tiles_kernel<PAIR, GATHER, GATED, TC>;
     if (!f8_configure<kernel, C::SMEM>()) return AIEN_E_STATE;

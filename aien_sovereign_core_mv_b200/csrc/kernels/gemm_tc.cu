@@ -468,7 +468,9 @@ static int launch_tc_grouped(const void* A, long lda, int rows_a, const void* W,
 // bank twice) and one lane issues the copy; rows and columns beyond the matrix are clipped by it.  Stored from registers,
 // every lane writes a row of its own, 16 bytes of 32 rows an instruction, and a sector of memory is written in two halves:
 // 2,048 x 8,192 x 2,048 took 68 us in float32 and 52 in bfloat16; 55 so (2,000 x 4,384 x 2,048: 37, now 29; 2,048 x 4,096 x 384: 17, now 11).
+// A copy writes whole 16-byte words: a box in which rows end inside one would take what lies behind them along, and is stored from registers.
 constexpr int TC_STORE_BYTES = 32 * 32 * 4, TC_STORE_BUFS = 8;               // of a CTA, dealt out to its epilogue warps
+__device__ __forceinline__ bool tc_box_leaves(int x, int N) { return (N & 3) == 0 || x + 32 <= N; }
 
 __device__ __forceinline__ void tc_store_tma(const uint32_t (&r)[32], uint32_t buf, const CUtensorMap* map, int lane, int x, int y, int z) {
 #pragma unroll
@@ -597,7 +599,7 @@ gemm_tc_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
                 uint32_t r[32];
                 tmem_ld32(tmem_acc + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * (P::TMEM_COLS / 2) + c0), r);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (sizeof(TC) == 4 && EPI == 0 && by_tma) {
+                if (sizeof(TC) == 4 && EPI == 0 && by_tma && tc_box_leaves(n0 + c0, N)) {
                     if (n0 + c0 >= N || m0 + quarter * 32 >= M) continue;
                     if (lane == 0) tma_store_read<1>();                // this warp's two buffers in turn: the older copy has read its own
                     __syncwarp();
@@ -906,7 +908,7 @@ gemm_tc_persistent_m256_kernel(const __grid_constant__ CUtensorMap map_a, const 
                 uint32_t r[32];
                 tmem_ld32(tmem_acc + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * P::BN + c0), r);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (sizeof(TC) == 4 && EPI == 0 && P::BN % 32 == 0 && by_tma) {
+                if (sizeof(TC) == 4 && EPI == 0 && P::BN % 32 == 0 && by_tma && tc_box_leaves(n0 + c0, N)) {
                     if (n0 + c0 >= N || m0 + quarter * 32 >= M) continue;
                     if (lane == 0) tma_store_read<0>();                // the warp's copy before has read the buffer
                     __syncwarp();
@@ -941,8 +943,7 @@ static int tc_num_sms() {
 // Whether a product's float32 results can leave by TMA (see tc_store_tma), and the map for them.
 template <int EPI, typename TC>
 static int tc_store_map(CUtensorMap* map, const void* out, long ldc, int M, int N, int parts, size_t part_stride) {
-    // (the copy writes whole 16-byte words: a row that ends inside one would take what lies behind it along)
-    if (sizeof(TC) != 4 || EPI != 0 || (ldc & 3) || (N & 3) || (part_stride & 3) || ((uintptr_t)out & 15)) return 0;
+    if (sizeof(TC) != 4 || EPI != 0 || (ldc & 3) || (part_stride & 3) || ((uintptr_t)out & 15)) return 0;
     return make_map_store_f32(map, out, (uint64_t)M, (uint64_t)N, (uint64_t)ldc, (uint64_t)parts, (uint64_t)part_stride) ? 1 : 0;
 }
 
