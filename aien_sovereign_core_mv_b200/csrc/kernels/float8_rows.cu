@@ -1,8 +1,8 @@
 // Numbers in 8 bits (e4m3) with one float32 scale for each block of 128: rows (a norm's, a gated activation's, any) and weights
 // in blocks of 128 x 128.
 //
-// A block with largest magnitude m gets the scale s = max(m / 448, 2^-126) and the codes e4m3(x * (1 / s)), to the nearest, ties to
-// even, at most 448.  A block of zeros has codes 0; a block that holds an infinity or something that is not a number has a
+// A block with largest magnitude m gets the scale s = max(m * (1 / 448), 2^-126) and the codes e4m3(x * (1 / s)), to the nearest, ties to
+// even, at most 448; both reciprocals and both products are rounded to float32.  A block of zeros has codes 0; a block that holds an infinity or something that is not a number has a
 // scale and codes that are not numbers, so that a product's row shows it as the product of the unscaled row would.
 // Largest magnitudes are taken over the bits of |x| as whole numbers: that order is the order of the numbers, and
 // what is not a number comes out above infinity instead of being lost.
@@ -56,7 +56,7 @@ __device__ __forceinline__ void f8_load8(const T* p, float v[8]) {
 // Where the eight numbers of a lane come from.  Eight neighbours, loaded whole, where every row starts on a 16-byte border and holds whole eights (load and
 // get); otherwise numbers lane, lane + 16, ... of the block, one by one (each).
 template <typename T> struct F8Plain {
-    static constexpr int CTAS = 8;                                             // on an SM: 32 registers a thread, 8,192 x 4,096 in 18.3 us for 19.6 with 40
+    static constexpr int CTAS = 8;                                             // on an SM: 32 registers a thread, 8,192 x 4,096 in 18.7 us for 19.6 with 40
     static constexpr float SIGN = 1.0f;
     const T* x;
     long ld;
@@ -108,8 +108,8 @@ __device__ __forceinline__ void f8_store(uint8_t* codes, int k0, int lane, int K
 }
 
 // Half a warp takes a block of a row, U blocks of it one after the other whose loads are all on their way first.  A CTA's 16 halves are `rows` (2^rows_log2) rows times
-// 16 / rows neighbouring blocks: one row where it has sixteen blocks, so that what a CTA reads lies together (gated, 512 x 12,288 in 7.6 us;
-// two rows of eight 7.8, eight rows of two, whose scales leave together, 8.1).
+// 16 / rows neighbouring blocks: one row where it has sixteen blocks, so that what a CTA reads lies together (gated, 512 x 12,288 in 8.3 us;
+// two rows of eight 8.4, eight rows of two, whose scales leave together, 8.6).
 // (As many CTAs as the GPU holds, walking over the blocks with the next one's numbers on their way, took longer: 2,048 x 12,288 gated in 37 us for 31.)
 template <typename SRC, bool VEC, int U>
 __global__ void __launch_bounds__(256, SRC::CTAS)
@@ -164,8 +164,8 @@ static int launch_rows_float8_by(SRC src, uint8_t* codes, long ldq, float* scale
     launch_chain(rows_float8_kernel<SRC, VEC, U>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, stream, src, codes, ldq, scales, lds, T, K, rows_log2);
     return launch_status();
 }
-// Two blocks a half from two loads of the GPU on (148 SMs of 128 halves): gated, 2,048 x 12,288 in 26.4 us by one and 23.9 by two, 512 x 12,288 in 8.0 and
-// 7.6, but 64 x 12,288 in 2.3 and 2.7; rows of 2,048 x 4,096 in 7.3 and 6.2, of 512 x 4,096 in 3.0 and 3.2.
+// Two blocks a half from two loads of the GPU on (148 SMs of 128 halves): gated, 2,048 x 12,288 in 29.4 us by one and 25.0 by two, 512 x 12,288 in 8.7 and
+// 8.3, but 64 x 12,288 in 2.5 and 3.0; rows of 2,048 x 4,096 in 6.5 and 6.2, of 512 x 4,096 in 2.5 and 2.9.
 template <typename SRC>
 static int launch_rows_float8(bool vec, SRC src, uint8_t* codes, long ldq, float* scales, long lds, int T, int K, cudaStream_t stream) {
     if (!vec) return launch_rows_float8_by<SRC, false, 1>(src, codes, ldq, scales, lds, T, K, stream);

@@ -2463,8 +2463,8 @@ def matrix_memory_chunked(proj: torch.Tensor, q_off: int, k_off: int, v_off: int
 
 # ---------------------------------------------------------------------------- linear layers in 8 bits
 # Numbers in 8 bits are e4m3 codes with one float32 scale for each block of 128: of a row's 128 neighbours, or of 128 x 128 numbers of a
-# weight.  scale = max|x| / 448, at least 2^-126; code = e4m3(x / scale), to the nearest (the reciprocal of the scale is rounded to
-# float32 first), at most 448.  A block that holds an infinity or something that is not a number has a scale and codes that are not
+# weight.  scale = max|x| times 1 / 448, at least 2^-126; code = e4m3(x times 1 / scale), to the nearest, at most 448 (both reciprocals and
+# both products are rounded to float32).  A block that holds an infinity or something that is not a number has a scale and codes that are not
 # numbers.  Codes [rows, K] may have a row stride; a last block may be short.  Scales of rows are laid out [ceil(K / 128), rows],
 # scales of a weight [ceil(N / 128), ceil(K / 128)]; both may have a row stride.
 FLOAT8_BLOCK = 128
